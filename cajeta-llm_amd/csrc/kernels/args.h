@@ -299,3 +299,33 @@ typedef struct {
     int32_t type;
     int32_t pad;
 } cj_moe_args;
+
+// K/V pages held in 8 bits (kv8.hip). A plane: codes, then one f32 scale for
+// each block of 16 positions of a kv head ([page][kv head][4]). K codes are
+// [page][kv head][64 positions][head_dim], V codes [page][kv head][4 blocks]
+// [head_dim][16 positions]; a code is its byte less 128, a value code · scale.
+// segs: {slot, first position, first row, rows} for each of n_segs segments.
+typedef struct {
+    const float *q, *k, *v;  // append: fresh rows; attend: q rows
+    float *q_out;            // append: rotated q rows (null: none)
+    float *out;              // attend: output rows; read: K rows (null: none)
+    float *out2;             // read: V rows (null: none)
+    uint8_t *kc, *vc;        // codes of the planes
+    float *ks, *vs;          // their scales
+    const float *qw, *kw;    // append: per-head norm weights (norm != 0)
+    const float *rope_cs;    // append: [rope_ctx][half] (cos, sin)
+    const int32_t *pgtab;    // [n_slots][slot_pages]
+    const int32_t *segs;
+    int32_t *status;         // set to 1 on a refused segment, page or value (may be null)
+    float *part;             // attend: partial results of the splits
+    int64_t q_stride, kv_stride, out_stride;   // floats between rows (append: out_stride is q_out's)
+    int32_t n_segs, max_rows, n_rows;          // rows of one segment and of the row buffers at most
+    int32_t limit;           // positions a segment may end at
+    int32_t n_pages, n_slots, slot_pages;
+    int32_t n_q, n_kv;
+    int32_t norm, form;
+    int32_t window;          // attend: positions a row sees (0: all before it)
+    int32_t splits, split_pages;               // attend: splits a segment at most, and pages of one
+    int32_t per_seg, kv_wgs;                   // append: workgroups of a segment's q rows; of all K/V blocks
+    float eps, scale;
+} cj_kv8_args;

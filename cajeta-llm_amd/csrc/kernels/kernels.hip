@@ -6,3 +6,4 @@
 #include "gemm.hip"
 #include "tile.hip"
 #include "rows.hip"
+#include "kv8.hip"

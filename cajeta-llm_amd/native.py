@@ -63,6 +63,11 @@ SIGNATURES = {
     "cj_argmax_row_noalloc": (I32, [I64, I32, I64, I64]),
     "cj_router_topk": (I32, [I64, I64, I64, I64, I64, I64, I32, I32, I32, I32, F32]),
     "cj_attn_scores": (I32, [I64, I64, I64, I64, I32, I32, I32, I32, I32, I32, F32]),
+    "cj_kv8_plane_bytes": (I64, [I32, I32, I32]),
+    "cj_kv8_append": (I32, [I64] * 11 + [I32] * 10 + [I64] * 3 + [I32, F32, I32, I64]),
+    "cj_kv8_read": (I32, [I64] * 6 + [I32] * 8 + [I64, I64]),
+    "cj_kv8_attend_bytes": (I64, [I32] * 7),
+    "cj_kv8_attend": (I32, [I64] * 7 + [I32] * 10 + [I64, I64, I32, F32, I64]),
     "cj_engine_load": (I64, [CP, I32, I32]),
     "cj_engine_load_kv": (I64, [CP, I32, I32, I32, I32]),
     "cj_engine_close": (I32, [I64]),

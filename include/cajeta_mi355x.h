@@ -262,6 +262,77 @@ int32_t cj_router_topk(int64_t sel, int64_t w, int64_t logits, int64_t w_router,
 int32_t cj_attn_scores(int64_t scores, int64_t q, int64_t kcache, int64_t pgtab, int32_t pg_base, int32_t n_q,
                        int32_t n_kv, int32_t head_dim, int32_t count, int32_t from, float scale);
 
+/* ------------------------------------------- K/V pages held in 8 bits */
+
+/* No counterpart in the reference (its planes hold fp16 or f32): the same
+ * pages of 64 positions at half the bytes, for any mixture of sequences.
+ *
+ * A plane (K or V) of n_pages pages holds an 8-bit code for each value and
+ * one f32 scale, a power of two, for each block of 16 positions of a kv
+ * head: codes [page][kv head][64][head_dim] for K, [page][kv head][4 blocks]
+ * [head_dim][16] for V, then scales [page][kv head][4]. A code is its byte
+ * less 128 (-127..127), a value code x scale. A block's scale is the least
+ * 2^e >= 2^-48 that holds its values; values appended into a block rescale
+ * its older codes where they need a larger one, so a stored value is off by
+ * less than one step of the block's scale (half a step when the block was
+ * filled by one call). A value that is not finite, or beyond 127 x 2^63,
+ * makes its block's scale NaN (rows that attend it come out NaN) and sets
+ * `status`.
+ *
+ * The calls work on n_segs segments: device int32 {slot, pos, row, rows}
+ * each: rows row .. row + rows of the row buffers are the positions pos ..
+ * pos + rows of the sequence in `slot`, whose pages stand in pgtab[slot]
+ * [0 .. slot_pages), one of [n_slots][slot_pages] rows. A segment may hold
+ * no rows; rows of no segment are left as they are. The segments and the
+ * page table are read on the device in stream order, so a captured graph
+ * follows their contents. A segment outside its bounds (slot < n_slots, rows
+ * <= max_rows, row + rows <= n_rows, positions within the slot's pages) is
+ * skipped and its rows left as they are; a page outside [0, n_pages) is not
+ * written, and read as NaN; either sets the int32 at `status` (a buffer
+ * handle, or 0 for none) to 1. Row buffers are f32, 16-byte aligned, strides
+ * in floats and multiples of 4. head_dim 64 or 128. */
+
+/* Bytes of one plane. */
+int64_t cj_kv8_plane_bytes(int32_t n_pages, int32_t n_kv, int32_t head_dim);
+
+/* The fresh rows of q, k and v: q and k normed per head (norm != 0; weights
+ * qw, kw, form 0: w, 1: 1 + w) and rotated (split halves, the positions'
+ * entries of the cj_rope_table with rope_ctx positions), q to q_out (which
+ * may be q; both 0: no queries), k and v into their pages. Arithmetic in 64
+ * bits, so codes are those of the exact values. A slot's positions from
+ * pos + rows on are dropped: their codes in the last block may change. A
+ * slot has at most one segment with rows in a call (of a slot with more, no
+ * k and v are appended, and `status` is set), and a page that is appended to
+ * belongs to one slot. Beside cj_qk_prep (one row, fp16 planes). */
+int32_t cj_kv8_append(int64_t q_out, int64_t q, int64_t k, int64_t v, int64_t kplane, int64_t vplane, int64_t qw, int64_t kw,
+                      int64_t rope, int64_t pgtab, int64_t segs, int32_t n_segs, int32_t max_rows, int32_t n_rows,
+                      int32_t rope_ctx, int32_t n_pages, int32_t n_slots, int32_t slot_pages, int32_t n_q, int32_t n_kv,
+                      int32_t head_dim, int64_t q_out_stride, int64_t q_stride, int64_t kv_stride, int32_t norm, float eps,
+                      int32_t form, int64_t status);
+
+/* The segments' positions as f32 rows of n_kv x head_dim values, K to k_out
+ * and V to v_out (one may be 0). */
+int32_t cj_kv8_read(int64_t k_out, int64_t v_out, int64_t kplane, int64_t vplane, int64_t pgtab, int64_t segs, int32_t n_segs,
+                    int32_t max_rows, int32_t n_rows, int32_t n_pages, int32_t n_slots, int32_t slot_pages, int32_t n_kv,
+                    int32_t head_dim, int64_t out_stride, int64_t status);
+
+/* Causal attention of the segments' q rows over their cached positions: the
+ * row at position p attends [max(0, p + 1 - window), p] (window 0: all), its
+ * own position, appended before, included; query head h reads kv head
+ * h / (n_q / n_kv). No segment ends past max_count. `part` holds the partial
+ * results where the positions are split over workgroups:
+ * cj_kv8_attend_bytes bytes (with the same arguments; 0: none, and part may
+ * be 0). Accurate to f32: the rows and weights enter the f16 matrix cores as
+ * two halves each, codes are exact in f16. Segments of one row and long
+ * chunks may share a call; each is fastest in a call of its own kind.
+ * Beside cj_attend (one row of one sequence, fp16 planes). */
+int64_t cj_kv8_attend_bytes(int32_t n_segs, int32_t max_rows, int32_t max_count, int32_t n_q, int32_t n_kv, int32_t head_dim,
+                            int32_t window);
+int32_t cj_kv8_attend(int64_t out, int64_t q, int64_t kplane, int64_t vplane, int64_t pgtab, int64_t segs, int64_t part,
+                      int32_t n_segs, int32_t max_rows, int32_t n_rows, int32_t max_count, int32_t n_pages, int32_t n_slots,
+                      int32_t slot_pages, int32_t n_q, int32_t n_kv, int32_t head_dim, int64_t q_stride, int64_t out_stride,
+                      int32_t window, float scale, int64_t status);
+
 /* ------------------------------------------------------------ engine */
 
 /* The LlmEngine surface (LlmEngine.cajeta:165-546) over a GGUF model:

@@ -121,3 +121,19 @@ def test_crafted_gguf_headers_are_refused_not_trusted(pkg, tmp_path):
         else:
             assert rc == pkg.native.CJ_ERR_IO, (name, rc)
             assert pkg.native.last_error(), name
+
+
+def test_kv8_sizes_and_refusals_without_a_gpu(pkg):
+    """The 8-bit planes' sizes, and shapes that the host refuses before it looks at a buffer."""
+    lib, ARG, STATE = pkg.native.lib(), pkg.native.CJ_ERR_ARG, pkg.native.CJ_ERR_STATE
+    assert lib.cj_kv8_plane_bytes(3, 8, 128) == 3 * 8 * (64 * 128 + 16)
+    assert lib.cj_kv8_plane_bytes(1 << 24, 8, 128) == (1 << 27) * (64 * 128 + 16)
+    assert lib.cj_kv8_plane_bytes(0, 8, 128) < 0 and lib.cj_kv8_plane_bytes(3, 8, 96) < 0
+    assert lib.cj_kv8_attend_bytes(1, 1, 4096, 32, 8, 128, 0) >= 0
+    for bad in ((0, 1, 64, 8, 2, 64, 0), (1, 0, 64, 8, 2, 64, 0), (1, 1, 0, 8, 2, 64, 0), (1, 1, 64, 7, 2, 64, 0),
+                (1, 1, 64, 8, 2, 80, 0), (1, 1, 64, 8, 2, 64, -1), (1, 1, 64, 130, 2, 64, 0)):
+        assert lib.cj_kv8_attend_bytes(*bad) == ARG, bad
+    good = [0] * 7 + [1, 1, 1, 64, 1, 1, 1, 8, 2, 64, 512, 512, 0, 0.1, 0]
+    assert lib.cj_kv8_attend(*good) == STATE
+    for at, v in ((7, 0), (8, 0), (9, -1), (11, 0), (12, 0), (13, 0), (13, 1 << 30), (14, 9), (15, 0), (16, 100)):
+        assert lib.cj_kv8_attend(*(good[:at] + [v] + good[at + 1:])) == ARG, (at, v)
