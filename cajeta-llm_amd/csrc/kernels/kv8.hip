@@ -306,66 +306,329 @@ DEV void kv8_read(const cj_kv8_args &a) {
         }
 }
 
-// Attention, one wave a (row, query head): a page's 64 positions a pass, a
-// lane a position for the scores, then lanes over the channels.
+// ------------------------------------------------------------- attention
+//
+// Softmax over the positions with running maxima, split over workgroups and
+// joined by cj_kv8_join. The f16 matrix cores carry both products at f32's
+// accuracy: codes are whole numbers up to 127, exact in f16, and q and the
+// weights enter as two f16 halves each (hi + lo, 22 bits).
+//
+// The block's V scale 2^e rides on the weight: with s the score in base 2 the
+// weight is w = 2^(s + e − M + 14), M the running maximum of ceil(s + e), so
+// that the output is Σ w·code / Σ w·2^−e. A whole M makes every rescaling
+// exact; 14 keeps the lo halves of all weights down to 2^-17 of the largest
+// out of f16's subnormals.
+
+typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
+
+#define KV8_LOG2E 1.44269504088896340736f
+#define KV8_WEIGHT 14.0f
+
+// Eight code bytes as f16: 0x64xx is 1024 + xx.
+DEV h16x8 kv8_half8(uint32_t a, uint32_t b) {
+    union { uint32_t u[4]; h16x8 h; } r;
+    r.u[0] = __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u);
+    r.u[1] = __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u);
+    r.u[2] = __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u);
+    r.u[3] = __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u);
+    return r.h - (_Float16)1152.0f;
+}
+
+// x as hi + lo halves.
+DEV void kv8_halves(const float (&x)[8], h16x8 &hi, h16x8 &lo) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        hi[i] = (_Float16)x[i];
+        lo[i] = (_Float16)__builtin_fmaf((float)hi[i], -1.0f, x[i]);
+    }
+}
+
+// The exponent of a block's scale as a float; NaN where the scale is.
+DEV float kv8_exp_f(float s) { return (float)((int)((__float_as_uint(s) >> 23) & 255u) - 127) + s * 0.0f; }
+DEV float kv8_recip(float s) { return __uint_as_float((254u << 23) - (__float_as_uint(s) & 0x7f800000u)); }
+
+// A column's q, an exponent k apart from [1, 2)·2^14: the factor that the
+// scores take back, scale·log2(e)·2^(k − 14).
+DEV int kv8_q_exponent(float top) { return (int)(__float_as_uint(top) >> 23) - 127; }
+
+DEV float kv8_max4(float v) {   // over the lanes l, l ^ 16, l ^ 32, l ^ 48
+    int a, b;
+    swap16(__float_as_int(v), a, b);
+    v = fmaxf(__int_as_float(a), __int_as_float(b));
+    swap32(__float_as_int(v), a, b);
+    return fmaxf(__int_as_float(a), __int_as_float(b));
+}
+DEV float kv8_sum4(float v) {
+    int a, b;
+    swap16(__float_as_int(v), a, b);
+    v = __int_as_float(a) + __int_as_float(b);
+    swap32(__float_as_int(v), a, b);
+    return __int_as_float(a) + __int_as_float(b);
+}
+
+// The pages [p0, p1) that split sp of the segment's rows r0 .. r1 covers, and
+// how many splits these rows have.
+DEV int kv8_split(const cj_kv8_args &a, const Kv8Seg &g, int r0, int r1, int sp, int &p0, int &p1) {
+    const int lo = a.window > 0 && g.pos + r0 >= a.window ? (g.pos + r0 + 1 - a.window) / KV8_PAGE : 0;
+    const int n = (g.pos + r1) / KV8_PAGE + 1 - lo;
+    p0 = lo + min(n, sp * a.split_pages);
+    p1 = lo + min(n, (sp + 1) * a.split_pages);
+    return (n + a.split_pages - 1) / a.split_pages;
+}
+
+// A split's results: [segment][kv head][column tile][split] of KV8_FEW columns
+// (HD sums each), then their maxima and sums of weights.
+#define KV8_FEW 16
 template <int HD>
-DEV void kv8_attend_row(const cj_kv8_args &a) {
-    __shared__ float sq[HD], sp[KV8_PAGE];
-    const int t = threadIdx.x, h = blockIdx.x % a.n_q, w = blockIdx.x / a.n_q, i = w % a.max_rows, s = w / a.max_rows;
+DEV float *kv8_part(const cj_kv8_args &a, int s, int h, int ct, int sp) {
+    return a.part + ((((int64_t)s * a.n_kv + h) * a.col_tiles + ct) * a.splits + sp) * (KV8_FEW * (HD + 2));
+}
+
+// Few columns (a column is a row and one query head of the kv head's group):
+// a workgroup a (segment, kv head, 16 columns, split), its four waves a page
+// each in turn. All operands come straight from memory to registers, in the
+// order that makes the scores' accumulators the next product's operand:
+//  - scores: A rows are keys, row m of tile t is position (m/4)·16 + 4t + m%4
+//    of the page, so lane group g = l/16 gets its 16 positions of block g in
+//    order, and one K and one V scale a lane;
+//  - output: B is the weights as they lie, A the V codes, 16 positions of a
+//    channel in 16 bytes.
+template <int HD>
+DEV void kv8_attend_few(const cj_kv8_args &a) {
+    constexpr int KS = HD / 32, DT = HD / 16, KW = HD / 64;   // steps over the channels; channel tiles; 16-byte words a lane and key
+    __shared__ __align__(16) float so[4][KV8_FEW][HD + 4];
+    __shared__ float sm[4][KV8_FEW], sl[4][KV8_FEW];
+    const int t = threadIdx.x, l = t & 63, wv = t >> 6, n = l & 15, g4 = l >> 4;
+    // workgroups eight apart share an L2: a segment's column tiles follow one another there
+    const int64_t id = blockIdx.x, per = id / (8 * a.col_tiles), rest = per * 8 + id % 8;
+    const int ct = (int)((id / 8) % a.col_tiles);
+    const int h = (int)(rest % a.n_kv), sp = (int)((rest / a.n_kv) % a.splits), s = (int)(rest / a.n_kv / a.splits);
     Kv8Seg g;
-    if (!kv8_seg(a, s, g) || i >= g.rows) return;
-    const int kvh = h / (a.n_q / a.n_kv), last = g.pos + i;
-    const int first = a.window > 0 && last >= a.window ? last + 1 - a.window : 0;
-    for (int d = t; d < HD; d += 64) sq[d] = a.q[(int64_t)(g.row + i) * a.q_stride + (int64_t)h * HD + d] * a.scale;
-    __syncthreads();
-    float m = -INFINITY, l = 0, acc[HD / 64] = {};
-    for (int pi = first / KV8_PAGE; pi <= last / KV8_PAGE; pi++) {
-        int page = kv8_page(a, g.slot, pi);
-        const bool bad = page < 0;
-        if (bad) {
-            page = 0;
-            if (a.status && t == 0) *a.status = 1;
+    if (s >= a.n_segs || !kv8_seg(a, s, g)) return;
+    const int grp = a.n_q / a.n_kv, cols = g.rows * grp, c0 = ct * KV8_FEW;
+    if (c0 >= cols) return;
+    const int r0 = c0 / grp, r1 = min(c0 + KV8_FEW, cols) - 1;   // (r1: a column here)
+    int p0, p1;
+    const int splits = kv8_split(a, g, r0, r1 / grp, sp, p0, p1);
+    if (sp >= splits) return;
+
+    // this lane's column (past the last: the tile's first again), and its q as halves
+    const int c = c0 + n < cols ? c0 + n : c0, ri = c / grp;
+    const int last = g.pos + ri, first = a.window > 0 ? last + 1 - a.window : 0;
+    h16x8 qh[KS], ql[KS];
+    float cs;
+    {
+        float x[KS][8], top = 0;
+        const float *src = a.q + (int64_t)(g.row + ri) * a.q_stride + (int64_t)(h * grp + c % grp) * HD + g4 * (HD / 4);
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            *(f32x4 *)&x[k][0] = *(const f32x4 *)(src + 8 * k);
+            *(f32x4 *)&x[k][4] = *(const f32x4 *)(src + 8 * k + 4);
+#pragma unroll
+            for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[k][i]));
         }
-        const int64_t ph = (int64_t)page * a.n_kv + kvh;
-        const float none = __uint_as_float(0x7fc00000u);
-        const int p = pi * KV8_PAGE + t;
-        const bool seen = p >= first && p <= last;
-        float x = 0;
-        const uint32_t *kr = (const uint32_t *)(a.kc + (ph * KV8_PAGE + t) * HD);
-        for (int c = 0; c < HD / 4; c++) {
-            const uint32_t b = kr[c];
+        const int e = kv8_q_exponent(kv8_max4(top));
+        cs = ldexpf(a.scale * KV8_LOG2E, e - 14);
 #pragma unroll
-            for (int k = 0; k < 4; k++) x = fmaf(sq[4 * c + k], (float)((int)((b >> (8 * k)) & 255u) - 128), x);
-        }
-        x = seen ? x * (bad ? none : a.ks[ph * 4 + t / 16]) : -INFINITY;
-        const float mt = fmaxf(m, xmax64(x));
-        const float r = m == -INFINITY ? 0.0f : __expf(m - mt), e = seen ? __expf(x - mt) : 0.0f;
-        float sum = e;
+        for (int k = 0; k < KS; k++) {
 #pragma unroll
-        for (int k = 1; k < 64; k *= 2) sum += __shfl_xor(sum, k);
-        l = l * r + sum;
-        m = mt;
-        __syncthreads();
-        sp[t] = seen ? e * a.vs[ph * 4 + t / 16] : 0.0f;
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < HD / 64; c++) {
-            float y = 0;
-            for (int k = 0; k < KV8_PAGE; k++) {
-                const uint8_t *v = a.vc + ph * KV8_PAGE * HD + (int64_t)(k / 16) * HD * 16 + (c * 64 + t) * 16 + k % 16;
-                y = fmaf(sp[k], (float)((int)*v - 128), y);
-            }
-            acc[c] = acc[c] * r + y;
+            for (int i = 0; i < 8; i++) x[k][i] = ldexpf(x[k][i], 14 - e);
+            kv8_halves(x[k], qh[k], ql[k]);
         }
     }
+    f32x4 o[DT] = {};
+    float M = -INFINITY, L = 0;
+
+    const int key0 = (n >> 2) * 16 + (n & 3);
+    u32x4 kr[4][KW], vr[DT];
+    float ks, vs;
+    int pi = p0 + wv;
+    bool bad = false;
+    auto page_at = [&](int i) {
+        const int p = kv8_page(a, g.slot, i);
+        bad = p < 0;
+        return (int64_t)(bad ? 0 : p) * a.n_kv + h;
+    };
+    auto load_k = [&](int64_t ph) {
+        const uint8_t *b = a.kc + ph * (KV8_PAGE * HD) + key0 * HD + g4 * (HD / 4);
 #pragma unroll
-    for (int c = 0; c < HD / 64; c++)
-        a.out[(int64_t)(g.row + i) * a.out_stride + (int64_t)h * HD + c * 64 + t] = acc[c] / l;
+        for (int q = 0; q < 4; q++)
+#pragma unroll
+            for (int i = 0; i < KW; i++) kr[q][i] = __builtin_nontemporal_load((const u32x4 *)(b + q * 4 * HD + i * 16));
+        ks = a.ks[ph * 4 + g4];
+        if (bad) ks = __uint_as_float(0x7fc00000u);
+    };
+    auto load_v = [&](int64_t ph) {
+        const uint8_t *b = a.vc + ph * (KV8_PAGE * HD) + (g4 * HD + n) * 16;
+#pragma unroll
+        for (int j = 0; j < DT; j++) vr[j] = __builtin_nontemporal_load((const u32x4 *)(b + j * 256));
+        vs = a.vs[ph * 4 + g4];
+    };
+    int64_t ph = 0;
+    if (pi < p1) {
+        ph = page_at(pi);
+        load_k(ph);
+        load_v(ph);
+    }
+    for (; pi < p1; pi += 4) {
+        if (bad && a.status && l == 0) *a.status = 1;
+        f32x4 x[4] = {};
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                const u32x4 w = kr[q][k / 2];
+                const h16x8 f = k & 1 ? kv8_half8(w[2], w[3]) : kv8_half8(w[0], w[1]);
+                x[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, qh[k], x[q], 0, 0, 0);
+                x[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, ql[k], x[q], 0, 0, 0);
+            }
+        const float kf = ks * cs, ve = kv8_exp_f(vs), vi = kv8_recip(vs);
+        const bool more = pi + 4 < p1;
+        if (more) {
+            ph = page_at(pi + 4);
+            load_k(ph);
+        }
+        float top = -INFINITY;
+        const int at = pi * KV8_PAGE + g4 * 16;
+        if (pi * KV8_PAGE + KV8_PAGE - 1 > g.pos + r0 || (a.window > 0 && pi * KV8_PAGE < g.pos + r1 / grp + 1 - a.window)) {
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int p = at + 4 * q + i;
+                    x[q][i] = p <= last && p >= first ? __builtin_fmaf(x[q][i], kf, ve) : -INFINITY;
+                }
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[q][i] = __builtin_fmaf(x[q][i], kf, ve);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) top = fmaxf(top, x[q][i]);
+        const float Mn = fmaxf(M, ceilf(kv8_max4(top)));
+        const float base = (Mn == -INFINITY ? 0.0f : Mn) - KV8_WEIGHT;
+        if (__any(Mn != M)) {
+            const float r = exp2f(M - (base + KV8_WEIGHT));
+#pragma unroll
+            for (int j = 0; j < DT; j++) o[j] *= r;
+            L *= r;
+            M = Mn;
+        }
+        h16x8 wh[2], wl[2];
+        float sum = 0;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            float w[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                w[i] = __builtin_amdgcn_exp2f(x[2 * u + i / 4][i % 4] - base);
+                sum += w[i];
+            }
+            kv8_halves(w, wh[u], wl[u]);
+        }
+        L += sum == 0.0f ? 0.0f : sum * vi;
+#pragma unroll
+        for (int j = 0; j < DT; j++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const h16x8 f = kv8_half8(vr[j][2 * u], vr[j][2 * u + 1]);
+                o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, wh[u], o[j], 0, 0, 0);
+                o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, wl[u], o[j], 0, 0, 0);
+            }
+        if (more) load_v(ph);
+    }
+
+    // the four waves' results as one
+    L = kv8_sum4(L);
+#pragma unroll
+    for (int j = 0; j < DT; j++) *(f32x4 *)&so[wv][n][j * 16 + g4 * 4] = o[j];
+    if (g4 == 0) {
+        sm[wv][n] = M;
+        sl[wv][n] = L;
+    }
+    __syncthreads();
+    float *part = splits > 1 ? kv8_part<HD>(a, s, h, ct, sp) : nullptr;
+    for (int i = t; i < KV8_FEW * HD / 4; i += 256) {
+        const int k = i / (HD / 4), d = i % (HD / 4) * 4;
+        if (c0 + k >= cols) break;
+        const float m = fmaxf(fmaxf(sm[0][k], sm[1][k]), fmaxf(sm[2][k], sm[3][k])), z = m == -INFINITY ? 0.0f : m;
+        f32x4 y = {};
+        float b = 0;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float f = exp2f(sm[w][k] - z);
+            y += *(const f32x4 *)&so[w][k][d] * f;
+            b += sl[w][k] * f;
+        }
+        if (part) {
+            *(f32x4 *)(part + k * HD + d) = y;
+            if (d == 0) {
+                part[KV8_FEW * HD + 2 * k] = m;
+                part[KV8_FEW * HD + 2 * k + 1] = b;
+            }
+        } else {
+            const int cc = c0 + k;
+            *(f32x4 *)(a.out + (int64_t)(g.row + cc / grp) * a.out_stride + (int64_t)(h * grp + cc % grp) * HD + d) = y / b;
+        }
+    }
+}
+
+// The splits of a column as one row: a workgroup a (segment, kv head, column),
+// 256 / HD threads a channel over the splits in turn, joined in order.
+template <int HD>
+DEV void kv8_join(const cj_kv8_args &a) {
+    constexpr int W = 256 / (HD / 4);
+    __shared__ __align__(16) float so[W][HD];
+    __shared__ float sm[W], sl[W];
+    const int t = threadIdx.x, d = t % (HD / 4) * 4, w = t / (HD / 4);
+    const int grp = a.n_q / a.n_kv, most = a.max_rows * grp;
+    const int c = blockIdx.x % most, h = blockIdx.x / most % a.n_kv, s = blockIdx.x / most / a.n_kv;
+    Kv8Seg g;
+    if (!kv8_seg(a, s, g) || c >= g.rows * grp) return;
+    const int ct = c / KV8_FEW, k = c % KV8_FEW, c0 = ct * KV8_FEW;
+    int p0, p1;
+    const int splits = kv8_split(a, g, c0 / grp, (min(c0 + KV8_FEW, g.rows * grp) - 1) / grp, 0, p0, p1);
+    if (splits <= 1) return;
+    const float *part = kv8_part<HD>(a, s, h, ct, 0);
+    float M = -INFINITY, L = 0;
+    f32x4 y = {};
+    for (int sp = w; sp < splits; sp += W) {
+        const float *p = part + (int64_t)sp * (KV8_FEW * (HD + 2));
+        const float m = p[KV8_FEW * HD + 2 * k], b = p[KV8_FEW * HD + 2 * k + 1];
+        const f32x4 v = *(const f32x4 *)(p + k * HD + d);
+        const float Mn = fmaxf(M, m), z = Mn == -INFINITY ? 0.0f : Mn, f0 = exp2f(M - z), f1 = exp2f(m - z);
+        y = y * f0 + v * f1;
+        L = L * f0 + b * f1;
+        M = Mn;
+    }
+    *(f32x4 *)&so[w][d] = y;
+    if (d == 0) {
+        sm[w] = M;
+        sl[w] = L;
+    }
+    __syncthreads();
+    if (w) return;
+    for (int i = 1; i < W; i++) M = fmaxf(M, sm[i]);
+    const float z = M == -INFINITY ? 0.0f : M;
+    f32x4 r = {};
+    float b = 0;
+    for (int i = 0; i < W; i++) {
+        const float f = exp2f(sm[i] - z);
+        r += *(const f32x4 *)&so[i][d] * f;
+        b += sl[i] * f;
+    }
+    *(f32x4 *)(a.out + (int64_t)(g.row + c / grp) * a.out_stride + (int64_t)(h * grp + c % grp) * HD + d) = r / b;
 }
 
 extern "C" __global__ void __launch_bounds__(256) cj_kv8_append_h64(cj_kv8_args a) { kv8_append<64>(a); }
 extern "C" __global__ void __launch_bounds__(256) cj_kv8_append_h128(cj_kv8_args a) { kv8_append<128>(a); }
 extern "C" __global__ void __launch_bounds__(256) cj_kv8_read_h64(cj_kv8_args a) { kv8_read<64>(a); }
 extern "C" __global__ void __launch_bounds__(256) cj_kv8_read_h128(cj_kv8_args a) { kv8_read<128>(a); }
-extern "C" __global__ void __launch_bounds__(64) cj_kv8_attend_row_h64(cj_kv8_args a) { kv8_attend_row<64>(a); }
-extern "C" __global__ void __launch_bounds__(64) cj_kv8_attend_row_h128(cj_kv8_args a) { kv8_attend_row<128>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) cj_kv8_attend_few_h64(cj_kv8_args a) { kv8_attend_few<64>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) cj_kv8_attend_few_h128(cj_kv8_args a) { kv8_attend_few<128>(a); }
+extern "C" __global__ void __launch_bounds__(256) cj_kv8_join_h64(cj_kv8_args a) { kv8_join<64>(a); }
+extern "C" __global__ void __launch_bounds__(256) cj_kv8_join_h128(cj_kv8_args a) { kv8_join<128>(a); }

@@ -57,6 +57,23 @@ int run(const char *kernel, int32_t hd, int64_t grid, uint32_t block, const cj_k
     return launch((std::string(kernel) + "_h" + std::to_string(hd)).c_str(), (uint32_t)grid, block, 0, a);
 }
 
+// How a call's positions are split: over enough workgroups to fill the chip,
+// four pages (one a wave) at least.
+struct Plan {
+    int64_t col_tiles, splits, split_pages, bytes;
+};
+Plan plan_attend(int64_t n_segs, int64_t max_rows, int64_t max_count, int64_t n_q, int64_t n_kv, int64_t hd, int64_t window) {
+    Plan p;
+    p.col_tiles = (max_rows * (n_q / n_kv) + 15) / 16;
+    int64_t pages = (max_count + 63) / 64;
+    if (window) pages = std::min(pages, (window + max_rows) / 64 + 2);   // what the rows of a tile see together
+    const int64_t units = n_segs * n_kv * p.col_tiles, want = std::max<int64_t>(1, 3 * device_cus() / units);
+    p.split_pages = std::max<int64_t>(4, (pages + want - 1) / want);
+    p.splits = (pages + p.split_pages - 1) / p.split_pages;
+    p.bytes = p.splits > 1 ? units * p.splits * 16 * (hd + 2) * 4 : 0;
+    return p;
+}
+
 }  // namespace
 }  // namespace cj
 
@@ -118,7 +135,8 @@ int64_t cj_kv8_attend_bytes(int32_t n_segs, int32_t max_rows, int32_t max_count,
     if (!shape_ok(n_q, n_kv, head_dim) || n_segs <= 0 || max_rows <= 0 || max_count <= 0 || window < 0)
         return fail(CJ_ERR_ARG, "cj_kv8_attend_bytes: %d segments of %d rows, %d positions, heads %d/%d of size %d", n_segs,
                     max_rows, max_count, n_q, n_kv, head_dim);
-    return 0;
+    if (!ready()) return fail(CJ_ERR_STATE, "cj_init has not run");   // the split follows the device's size
+    return plan_attend(n_segs, max_rows, max_count, n_q, n_kv, head_dim, window).bytes;
 }
 
 int32_t cj_kv8_attend(int64_t out, int64_t q, int64_t kplane, int64_t vplane, int64_t pgtab, int64_t segs, int64_t part,
@@ -135,7 +153,16 @@ int32_t cj_kv8_attend(int64_t out, int64_t q, int64_t kplane, int64_t vplane, in
         return fail(CJ_ERR_ARG, "cj_kv8_attend: q or out is not %d rows of %lld floats, 16-byte aligned", n_rows, (long long)qn);
     a.q = (const float *)dptr(q); a.out = (float *)dptr(out); a.q_stride = q_stride; a.out_stride = out_stride;
     a.limit = std::min(a.limit, max_count); a.window = window; a.scale = scale;
-    return run("cj_kv8_attend_row", head_dim, (int64_t)n_segs * max_rows * n_q, 64, a);
+    const Plan p = plan_attend(n_segs, max_rows, max_count, n_q, n_kv, head_dim, window);
+    if (p.bytes && ((part & 15) || !in_buffer(dptr(part), p.bytes)))
+        return fail(CJ_ERR_ARG, "cj_kv8_attend: part is not 16-byte aligned or smaller than %lld bytes", (long long)p.bytes);
+    const int64_t wgs = ((int64_t)n_segs * n_kv * p.splits + 7) / 8 * 8 * p.col_tiles, join = (int64_t)n_segs * max_rows * n_q;
+    if (wgs > 0x7fffffff || join > 0x7fffffff)
+        return fail(CJ_ERR_ARG, "cj_kv8_attend: %d x %d rows of %d heads exceed a launch", n_segs, max_rows, n_q);
+    a.part = (float *)dptr(part); a.col_tiles = (int32_t)p.col_tiles; a.splits = (int32_t)p.splits;
+    a.split_pages = (int32_t)p.split_pages;
+    const int rc = run("cj_kv8_attend_few", head_dim, wgs, 256, a);
+    return rc || p.splits == 1 ? rc : run("cj_kv8_join", head_dim, join, 256, a);
 }
 
 }  // extern "C"

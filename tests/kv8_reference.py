@@ -52,6 +52,7 @@ class Cache:
         return x[first:first + count]
 
     def steps(self, slot, name):
+        """[block, kv]"""
         return np.stack([s for _, s in self._slot(slot)[name]])
 
 
@@ -67,14 +68,19 @@ def turned(x, rope, pos):
     return np.concatenate((a * c - b * s, a * s + b * c), -1)
 
 
-def attention(q, k, v, pos, scale, window=0):
-    """q [rows, heads, hd] at positions pos.. over k, v [positions, kv, hd]: the output and how far f32 may be from it.
+def attention(q, k, v, pos, scale, window, steps):
+    """q [rows, heads, hd] at positions pos.. over k, v [positions, kv, hd], `steps` [positions, kv] those of v's blocks:
+    the output and how far the attention may be from it.
 
     With u = 2^-24: a score's products and sums round hd + 4 times at most, the halves of q leave 2^-22 of each value, so
     a score is off by at most d = scale x sum|q k| x ((hd + 4) u + 2^-22), and the exponent's argument (in base 2, after
     it is scaled and the block's exponent, at most 64 here, is added) rounds three times. A weight is then off by the
     relative d + 3 u x (|s| + 64) x 1.5 + 2^-21 (exp2, the halves of the weight, the scales); the sums over n positions
-    round n times. Numerator and denominator both carry that."""
+    round n times. Numerator and denominator both carry that.
+
+    A weight times its block's step is held in two f16 halves, scaled so that the largest of the row lies in (2^13, 2^14]:
+    where the halves reach f16's subnormals, which are 2^-24 apart, it is off by up to 2^-25, that is 2^-38 of the largest;
+    each of the n positions' codes, 127 at most, may carry that."""
     rows, heads, hd = q.shape
     kv, u = k.shape[1], 2.0 ** -24
     out, tol = np.zeros((rows, heads, hd)), np.zeros((rows, heads, hd))
@@ -88,5 +94,6 @@ def attention(q, k, v, pos, scale, window=0):
             p /= p.sum()
             out[i, h] = p @ vv
             rel = big * ((hd + 4) * u + 2.0 ** -22) + 4.5 * u * (np.abs(s).max() * 1.5 + 64) + 2.0 ** -21 + (len(kk) + 8) * u
-            tol[i, h] = 2 * rel * (p @ np.abs(vv)) + 1e-30
+            held = (p * steps[lo:pos + i + 1, h * kv // heads]).max()
+            tol[i, h] = 2 * rel * (p @ np.abs(vv)) + len(kk) * 127 * 2.0 ** -38 * held + 1e-30
     return out, tol

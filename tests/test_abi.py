@@ -129,7 +129,7 @@ def test_kv8_sizes_and_refusals_without_a_gpu(pkg):
     assert lib.cj_kv8_plane_bytes(3, 8, 128) == 3 * 8 * (64 * 128 + 16)
     assert lib.cj_kv8_plane_bytes(1 << 24, 8, 128) == (1 << 27) * (64 * 128 + 16)
     assert lib.cj_kv8_plane_bytes(0, 8, 128) < 0 and lib.cj_kv8_plane_bytes(3, 8, 96) < 0
-    assert lib.cj_kv8_attend_bytes(1, 1, 4096, 32, 8, 128, 0) >= 0
+    assert lib.cj_kv8_attend_bytes(1, 1, 4096, 32, 8, 128, 0) == STATE
     for bad in ((0, 1, 64, 8, 2, 64, 0), (1, 0, 64, 8, 2, 64, 0), (1, 1, 0, 8, 2, 64, 0), (1, 1, 64, 7, 2, 64, 0),
                 (1, 1, 64, 8, 2, 80, 0), (1, 1, 64, 8, 2, 64, -1), (1, 1, 64, 130, 2, 64, 0)):
         assert lib.cj_kv8_attend_bytes(*bad) == ARG, bad

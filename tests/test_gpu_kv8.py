@@ -127,7 +127,8 @@ class Pages:
                 continue
             seen[row:row + cnt] = True
             want, tol = attention(q[row:row + cnt].astype(np.float64), self.ref.values(slot, "k", 0, pos + cnt),
-                                  self.ref.values(slot, "v", 0, pos + cnt), pos, scale, window)
+                                  self.ref.values(slot, "v", 0, pos + cnt), pos, scale, window,
+                                  self.ref.steps(slot, "v").repeat(BLOCK, 0))
             off = np.abs(got[row:row + cnt] - want)
             assert np.isfinite(got[row:row + cnt]).all(), (slot, pos, cnt)
             assert (off <= tol).all(), (slot, pos, cnt, float((off / tol).max()))
@@ -472,7 +473,7 @@ def test_a_captured_step_follows_its_segments_and_tables(gpu):
             P.ref.append(s, lens[s], turned(x[:, heads:heads + kv], P.rope, lens[s]), x[:, heads + kv:])
             qq = turned(x[:, :heads], P.rope, lens[s]).astype(np.float32).astype(np.float64)
             want, tol = attention(qq, P.ref.values(s, "k", 0, lens[s] + 1), P.ref.values(s, "v", 0, lens[s] + 1), lens[s],
-                                  np.float64(np.float32(1 / math.sqrt(hd))))
+                                  np.float64(np.float32(1 / math.sqrt(hd))), 0, P.ref.steps(s, "v").repeat(BLOCK, 0))
             # q's own rounding to f32 may fall the other way: 2^-23 of each value moves a score by that share of sum|q k|
             assert (np.abs(got.reshape(n, heads, hd)[i] - want[0]) <= 2 * tol[0]).all()
             lens[s] += 1
