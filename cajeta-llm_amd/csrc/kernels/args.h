@@ -326,7 +326,7 @@ typedef struct {
     int32_t norm, form;
     int32_t window;          // attend: positions a row sees (0: all before it)
     int32_t splits, split_pages;               // attend: splits of a segment's rows at most, and pages of one
-    int32_t col_tiles;       // attend: column tiles of a segment and kv head at most
+    int32_t col_tiles, tile_cols;              // attend: column tiles of a segment and kv head at most, columns of one
     int32_t per_seg, kv_wgs;                   // append: workgroups of a segment's q rows; of all K/V blocks
     float eps, scale;
 } cj_kv8_args;

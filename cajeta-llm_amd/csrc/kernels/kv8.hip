@@ -320,7 +320,8 @@ DEV void kv8_read(const cj_kv8_args &a) {
 // out of f16's subnormals.
 
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 #define KV8_LOG2E 1.44269504088896340736f
 #define KV8_WEIGHT 14.0f
@@ -377,12 +378,12 @@ DEV int kv8_split(const cj_kv8_args &a, const Kv8Seg &g, int r0, int r1, int sp,
     return (n + a.split_pages - 1) / a.split_pages;
 }
 
-// A split's results: [segment][kv head][column tile][split] of KV8_FEW columns
-// (HD sums each), then their maxima and sums of weights.
+// A split's results: [segment][kv head][column tile][split] of the tile's
+// columns (HD sums each), then their maxima and sums of weights.
 #define KV8_FEW 16
 template <int HD>
 DEV float *kv8_part(const cj_kv8_args &a, int s, int h, int ct, int sp) {
-    return a.part + ((((int64_t)s * a.n_kv + h) * a.col_tiles + ct) * a.splits + sp) * (KV8_FEW * (HD + 2));
+    return a.part + ((((int64_t)s * a.n_kv + h) * a.col_tiles + ct) * a.splits + sp) * (a.tile_cols * (HD + 2));
 }
 
 // Few columns (a column is a row and one query head of the kv head's group):
@@ -577,6 +578,211 @@ DEV void kv8_attend_few(const cj_kv8_args &a) {
     }
 }
 
+// Many columns (prefill chunks): a workgroup a (segment, kv head, 128 columns,
+// split), a wave 32 columns, every wave over the same pages. A page's codes
+// become f16 once, on their way into LDS, and serve the four waves; the next
+// page's codes are on their way to registers meanwhile, so a page costs one
+// barrier. As above, the tiles' rows are placed so that lane half h = l/32
+// gets blocks 2h and 2h + 1 of the page in order and the scores' accumulators
+// are the weights' operand as they lie.
+//  - K in LDS: row 32t + r of 16-byte words, word c at c ^ (row & 15), so that
+//    eight lanes' rows lie in different banks;
+//  - V in LDS: [t][u][h][channel] words of the 8 positions 8u.. of block 2h + t.
+#define KV8_MANY 128
+template <int HD>
+DEV void kv8_attend_many(const cj_kv8_args &a) {
+    constexpr int KS = HD / 16, DT = HD / 32, CH = HD / 64;   // steps, channel tiles, 16-byte words of codes a thread and plane
+    constexpr int ROW = HD * 2, BUF = KV8_PAGE * ROW;
+    __shared__ __align__(16) uint8_t sk[2][BUF], sv[2][BUF];
+    const int t = threadIdx.x, l = t & 63, wv = t >> 6, n = l & 31, hf = l >> 5;
+    const int64_t id = blockIdx.x;
+    const int h = (int)(id % a.n_kv), sp = (int)(id / a.n_kv % a.splits), s = (int)(id / a.n_kv / a.splits % a.n_segs);
+    const int ct = a.col_tiles - 1 - (int)(id / a.n_kv / a.splits / a.n_segs);   // the longest first
+    Kv8Seg g;
+    if (!kv8_seg(a, s, g)) return;
+    const int grp = a.n_q / a.n_kv, cols = g.rows * grp, c0 = ct * KV8_MANY;
+    if (c0 >= cols) return;
+    int p0, p1;
+    const int splits = kv8_split(a, g, c0 / grp, (min(c0 + KV8_MANY, cols) - 1) / grp, sp, p0, p1);
+    if (sp >= splits) return;
+
+    // the wave's columns, this lane's, and its q as halves (columns past the last: the last again)
+    const int w0 = min(c0 + wv * 32, cols - 1), w1 = min(c0 + wv * 32 + 31, cols - 1), c = min(c0 + wv * 32 + n, cols - 1), ri = c / grp;
+    const int wfirst = g.pos + w0 / grp, wlast = g.pos + w1 / grp, last = g.pos + ri, first = a.window > 0 ? last + 1 - a.window : 0;
+    const int wlow = a.window > 0 ? wfirst + 1 - a.window : 0;   // the first position that any column of the wave sees
+    h16x8 qh[KS], ql[KS];
+    float cs;
+    {
+        float x[KS][8], top = 0;
+        const float *src = a.q + (int64_t)(g.row + ri) * a.q_stride + (int64_t)(h * grp + c % grp) * HD + hf * 8;
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            *(f32x4 *)&x[k][0] = *(const f32x4 *)(src + 16 * k);
+            *(f32x4 *)&x[k][4] = *(const f32x4 *)(src + 16 * k + 4);
+#pragma unroll
+            for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[k][i]));
+        }
+        int u, v;
+        swap32(__float_as_int(top), u, v);
+        const int e = kv8_q_exponent(fmaxf(__int_as_float(u), __int_as_float(v)));
+        const float sign = a.scale < 0 ? -1.0f : 1.0f;
+        cs = ldexpf(a.scale * sign * KV8_LOG2E, e - 14);
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[k][i] = ldexpf(x[k][i] * sign, 14 - e);
+            kv8_halves(x[k], qh[k], ql[k]);
+        }
+    }
+    f32x16 o[DT] = {};
+    float M = -INFINITY, L = 0;
+
+    // staging: thread t moves words t, t + 256, .. of the page's K and V codes
+    u32x4 kr[CH], vr[CH];
+    f32x2 ksn, vsn;
+    bool bad = false;
+    auto load = [&](int i) {
+        const int p = kv8_page(a, g.slot, i);
+        bad = p < 0;
+        const int64_t ph = (int64_t)(bad ? 0 : p) * a.n_kv + h;
+        const u32x4 *kb = (const u32x4 *)(a.kc + ph * (KV8_PAGE * HD)), *vb = (const u32x4 *)(a.vc + ph * (KV8_PAGE * HD));
+#pragma unroll
+        for (int k = 0; k < CH; k++) {
+            kr[k] = kb[t + 256 * k];
+            vr[k] = vb[t + 256 * k];
+        }
+        ksn = *(const f32x2 *)(a.ks + ph * 4 + 2 * hf);
+        vsn = *(const f32x2 *)(a.vs + ph * 4 + 2 * hf);
+        if (bad) {
+            ksn[0] = ksn[1] = __uint_as_float(0x7fc00000u);
+            if (a.status && t == 0) *a.status = 1;
+        }
+    };
+    auto store = [&](int b) {
+#pragma unroll
+        for (int k = 0; k < CH; k++) {
+            const int w = t + 256 * k;
+            const int key = w / (HD / 16), c = w % (HD / 16) * 2;
+            const int row = (key >> 4 & 1) * 32 + (key >> 2 & 3) * 8 + (key >> 5) * 4 + (key & 3);
+            uint8_t *d = sk[b] + row * ROW;
+            *(h16x8 *)(d + ((c ^ row) & (HD / 8 - 1)) * 16) = kv8_half8(kr[k][0], kr[k][1]);
+            *(h16x8 *)(d + (((c + 1) ^ row) & (HD / 8 - 1)) * 16) = kv8_half8(kr[k][2], kr[k][3]);
+            const int blk = w / HD, ch = w % HD;
+            uint8_t *e = sv[b] + ((blk & 1) * 4 + (blk >> 1)) * (HD * 16) + ch * 16;
+            *(h16x8 *)e = kv8_half8(vr[k][0], vr[k][1]);
+            *(h16x8 *)(e + 2 * HD * 16) = kv8_half8(vr[k][2], vr[k][3]);
+        }
+    };
+    load(p0);
+    store(0);
+    f32x2 ks = ksn, vs = vsn;
+    for (int pi = p0, b = 0; pi < p1; pi++, b ^= 1) {
+        __syncthreads();   // the page is in buffer b; buffer b ^ 1 is free
+        const bool more = pi + 1 < p1;
+        if (more) load(pi + 1);
+        if (pi * KV8_PAGE <= wlast && pi * KV8_PAGE + KV8_PAGE > wlow) {
+            f32x16 x[2] = {};
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    const h16x8 f = *(const h16x8 *)(sk[b] + (32 * q + n) * ROW + (((2 * k + hf) ^ n) & (HD / 8 - 1)) * 16);
+                    x[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, qh[k], x[q], 0, 0, 0);
+                    x[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, ql[k], x[q], 0, 0, 0);
+                }
+            f32x2 kb = ks, vb = vs;
+            if (pi * KV8_PAGE + KV8_PAGE - 1 > wfirst || (a.window > 0 && pi * KV8_PAGE < wlast + 1 - a.window)) {
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    const int p = pi * KV8_PAGE + hf * 32 + q * 16;
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        if (p + i > last || p + i < first) x[q][i] = -INFINITY;
+                    if (p > last || p + 15 < first) kb[q] = vb[q] = 1.0f;   // a block that is not seen may have no scale
+                }
+            }
+            float kf[2], ve[2], top = -INFINITY;
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                kf[q] = kb[q] * cs;
+                kf[q] = kf[q] < 1e-37f ? 1e-37f : kf[q];   // (never zero: -inf stays -inf)
+                ve[q] = kv8_exp_f(vb[q]);
+                float m = x[q][0];
+#pragma unroll
+                for (int i = 1; i < 16; i++) m = fmaxf(m, x[q][i]);
+                top = fmaxf(top, __builtin_fmaf(m, kf[q], ve[q]));
+            }
+            int u, v;
+            swap32(__float_as_int(top), u, v);
+            const float Mn = fmaxf(M, ceilf(fmaxf(__int_as_float(u), __int_as_float(v))));
+            const float base = (Mn == -INFINITY ? 0.0f : Mn) - KV8_WEIGHT;
+            if (__any(Mn != M)) {
+                const float r = __builtin_amdgcn_exp2f(M - (base + KV8_WEIGHT));
+#pragma unroll
+                for (int j = 0; j < DT; j++) o[j] *= r;
+                L *= r;
+                M = Mn;
+            }
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                const float off = ve[q] - base;
+                h16x8 wh[2], wl[2];
+                float sum = 0;
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    float w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[q][8 * u + i], kf[q], off));
+                        sum += w[i];
+                    }
+                    kv8_halves(w, wh[u], wl[u]);
+                }
+                L += sum == 0.0f ? 0.0f : sum * kv8_recip(vb[q]);
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int j = 0; j < DT; j++) {
+                        const h16x8 f = *(const h16x8 *)(sv[b] + ((q * 2 + u) * 2 + hf) * (HD * 16) + (j * 32 + n) * 16);
+                        o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, wh[u], o[j], 0, 0, 0);
+                        o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, wl[u], o[j], 0, 0, 0);
+                    }
+            }
+        }
+        if (more) {
+            store(b ^ 1);
+            ks = ksn;
+            vs = vsn;
+        }
+    }
+    int u, v;
+    swap32(__float_as_int(L), u, v);
+    L = __int_as_float(u) + __int_as_float(v);
+    if (c0 + wv * 32 + n >= cols) return;
+    float *d;
+    if (splits > 1) {
+        const int k = wv * 32 + n;
+        float *part = kv8_part<HD>(a, s, h, ct, sp);
+        if (hf == 0) {
+            part[KV8_MANY * HD + 2 * k] = M;
+            part[KV8_MANY * HD + 2 * k + 1] = L;
+        }
+        d = part + k * HD;
+        L = 1.0f;
+    } else {
+        d = a.out + (int64_t)(g.row + ri) * a.out_stride + (int64_t)(h * grp + c % grp) * HD;
+    }
+#pragma unroll
+    for (int j = 0; j < DT; j++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            f32x4 y;
+#pragma unroll
+            for (int i = 0; i < 4; i++) y[i] = o[j][4 * q + i] / L;
+            *(f32x4 *)(d + j * 32 + q * 8 + hf * 4) = y;
+        }
+}
+
 // The splits of a column as one row: a workgroup a (segment, kv head, column),
 // 256 / HD threads a channel over the splits in turn, joined in order.
 template <int HD>
@@ -589,16 +795,16 @@ DEV void kv8_join(const cj_kv8_args &a) {
     const int c = blockIdx.x % most, h = blockIdx.x / most % a.n_kv, s = blockIdx.x / most / a.n_kv;
     Kv8Seg g;
     if (!kv8_seg(a, s, g) || c >= g.rows * grp) return;
-    const int ct = c / KV8_FEW, k = c % KV8_FEW, c0 = ct * KV8_FEW;
+    const int tc = a.tile_cols, ct = c / tc, k = c % tc, c0 = ct * tc;
     int p0, p1;
-    const int splits = kv8_split(a, g, c0 / grp, (min(c0 + KV8_FEW, g.rows * grp) - 1) / grp, 0, p0, p1);
+    const int splits = kv8_split(a, g, c0 / grp, (min(c0 + tc, g.rows * grp) - 1) / grp, 0, p0, p1);
     if (splits <= 1) return;
     const float *part = kv8_part<HD>(a, s, h, ct, 0);
     float M = -INFINITY, L = 0;
     f32x4 y = {};
     for (int sp = w; sp < splits; sp += W) {
-        const float *p = part + (int64_t)sp * (KV8_FEW * (HD + 2));
-        const float m = p[KV8_FEW * HD + 2 * k], b = p[KV8_FEW * HD + 2 * k + 1];
+        const float *p = part + (int64_t)sp * (tc * (HD + 2));
+        const float m = p[tc * HD + 2 * k], b = p[tc * HD + 2 * k + 1];
         const f32x4 v = *(const f32x4 *)(p + k * HD + d);
         const float Mn = fmaxf(M, m), z = Mn == -INFINITY ? 0.0f : Mn, f0 = exp2f(M - z), f1 = exp2f(m - z);
         y = y * f0 + v * f1;
@@ -632,3 +838,5 @@ extern "C" __global__ void __launch_bounds__(256, 2) cj_kv8_attend_few_h64(cj_kv
 extern "C" __global__ void __launch_bounds__(256, 2) cj_kv8_attend_few_h128(cj_kv8_args a) { kv8_attend_few<128>(a); }
 extern "C" __global__ void __launch_bounds__(256) cj_kv8_join_h64(cj_kv8_args a) { kv8_join<64>(a); }
 extern "C" __global__ void __launch_bounds__(256) cj_kv8_join_h128(cj_kv8_args a) { kv8_join<128>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) cj_kv8_attend_many_h64(cj_kv8_args a) { kv8_attend_many<64>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) cj_kv8_attend_many_h128(cj_kv8_args a) { kv8_attend_many<128>(a); }

@@ -57,20 +57,25 @@ int run(const char *kernel, int32_t hd, int64_t grid, uint32_t block, const cj_k
     return launch((std::string(kernel) + "_h" + std::to_string(hd)).c_str(), (uint32_t)grid, block, 0, a);
 }
 
-// How a call's positions are split: over enough workgroups to fill the chip,
-// four pages (one a wave) at least.
+// How a call runs: the column tiles of a segment (a column is a row and a
+// query head of one kv head's group), and the positions' split over enough
+// workgroups to fill the chip.
 struct Plan {
-    int64_t col_tiles, splits, split_pages, bytes;
+    bool many;
+    int64_t tile_cols, col_tiles, splits, split_pages, bytes;
 };
 Plan plan_attend(int64_t n_segs, int64_t max_rows, int64_t max_count, int64_t n_q, int64_t n_kv, int64_t hd, int64_t window) {
     Plan p;
-    p.col_tiles = (max_rows * (n_q / n_kv) + 15) / 16;
+    const int64_t cols = max_rows * (n_q / n_kv), cus = std::max(1, device_cus());
+    p.many = cols > 64;
+    p.tile_cols = p.many ? 128 : 16;
+    p.col_tiles = (cols + p.tile_cols - 1) / p.tile_cols;
     int64_t pages = (max_count + 63) / 64;
     if (window) pages = std::min(pages, (window + max_rows) / 64 + 2);   // what the rows of a tile see together
-    const int64_t units = n_segs * n_kv * p.col_tiles, want = std::max<int64_t>(1, 3 * device_cus() / units);
+    const int64_t units = n_segs * n_kv * p.col_tiles, want = std::max<int64_t>(1, (p.many ? 2 : 3) * cus / units);
     p.split_pages = std::max<int64_t>(4, (pages + want - 1) / want);
     p.splits = (pages + p.split_pages - 1) / p.split_pages;
-    p.bytes = p.splits > 1 ? units * p.splits * 16 * (hd + 2) * 4 : 0;
+    p.bytes = p.splits > 1 ? units * p.splits * p.tile_cols * (hd + 2) * 4 : 0;
     return p;
 }
 
@@ -156,12 +161,13 @@ int32_t cj_kv8_attend(int64_t out, int64_t q, int64_t kplane, int64_t vplane, in
     const Plan p = plan_attend(n_segs, max_rows, max_count, n_q, n_kv, head_dim, window);
     if (p.bytes && ((part & 15) || !in_buffer(dptr(part), p.bytes)))
         return fail(CJ_ERR_ARG, "cj_kv8_attend: part is not 16-byte aligned or smaller than %lld bytes", (long long)p.bytes);
-    const int64_t wgs = ((int64_t)n_segs * n_kv * p.splits + 7) / 8 * 8 * p.col_tiles, join = (int64_t)n_segs * max_rows * n_q;
+    const int64_t units = (int64_t)n_segs * n_kv * p.splits, join = (int64_t)n_segs * max_rows * n_q;
+    const int64_t wgs = (p.many ? units : (units + 7) / 8 * 8) * p.col_tiles;
     if (wgs > 0x7fffffff || join > 0x7fffffff)
         return fail(CJ_ERR_ARG, "cj_kv8_attend: %d x %d rows of %d heads exceed a launch", n_segs, max_rows, n_q);
-    a.part = (float *)dptr(part); a.col_tiles = (int32_t)p.col_tiles; a.splits = (int32_t)p.splits;
+    a.part = (float *)dptr(part); a.col_tiles = (int32_t)p.col_tiles; a.tile_cols = (int32_t)p.tile_cols; a.splits = (int32_t)p.splits;
     a.split_pages = (int32_t)p.split_pages;
-    const int rc = run("cj_kv8_attend_few", head_dim, wgs, 256, a);
+    const int rc = run(p.many ? "cj_kv8_attend_many" : "cj_kv8_attend_few", head_dim, wgs, 256, a);
     return rc || p.splits == 1 ? rc : run("cj_kv8_join", head_dim, join, 256, a);
 }
 
