@@ -305,6 +305,7 @@ typedef struct {
 // [page][kv head][64 positions][head_dim], V codes [page][kv head][4 blocks]
 // [head_dim][16 positions]; a code is its byte less 128, a value code · scale.
 // segs: {slot, first position, first row, rows} for each of n_segs segments.
+#define KV8_QS 4             // append: turns of 2048 / head_dim (row, query head) pairs of a workgroup
 typedef struct {
     const float *q, *k, *v;  // append: fresh rows; attend: q rows
     float *q_out;            // append: rotated q rows (null: none)
@@ -327,6 +328,7 @@ typedef struct {
     int32_t window;          // attend: positions a row sees (0: all before it)
     int32_t splits, split_pages;               // attend: splits of a segment's rows at most, and pages of one
     int32_t col_tiles, tile_cols;              // attend: column tiles of a segment and kv head at most, columns of one
+    int32_t join_ways;       // join: threads side by side over a column's splits (a power of two)
     int32_t per_seg, kv_wgs;                   // append: workgroups of a segment's q rows; of all K/V blocks
     float eps, scale;
 } cj_kv8_args;

@@ -41,8 +41,41 @@ DEV int kv8_page(const cj_kv8_args &a, int slot, int i) {
     return p >= 0 && p < a.n_pages ? p : -1;
 }
 
-DEV double kv8_shfl_xor(double v, int m) {
-    return __hiloint2double(__shfl_xor(__double2hiint(v), m), __shfl_xor(__double2loint(v), m));
+// Another lane's double by DPP, and the two halves of the exchanges with lane
+// ^ 16 and lane ^ 32. Pairs, quads, mirrored eights and mirrored rows: a sum
+// over 8 or 16 lanes, a maximum over all.
+template <int CTRL>
+DEV double kv8_dpp(double v) {
+    return __hiloint2double(dpp_i<CTRL>(__double2hiint(v)), dpp_i<CTRL>(__double2loint(v)));
+}
+#define KV8_MIRROR 0x140   // row_mirror
+template <int LANES>
+DEV double kv8_sum(double v) {
+    v += kv8_dpp<DPP_XOR1>(v);
+    v += kv8_dpp<DPP_XOR2>(v);
+    v += kv8_dpp<DPP_HMIRROR>(v);
+    return LANES == 8 ? v : v + kv8_dpp<KV8_MIRROR>(v);
+}
+DEV double kv8_max64(double v) {
+    v = fmax(v, kv8_dpp<DPP_XOR1>(v));
+    v = fmax(v, kv8_dpp<DPP_XOR2>(v));
+    v = fmax(v, kv8_dpp<DPP_HMIRROR>(v));
+    v = fmax(v, kv8_dpp<KV8_MIRROR>(v));
+    int a, b, c, d;
+    swap16(__double2hiint(v), a, b);
+    swap16(__double2loint(v), c, d);
+    v = fmax(__hiloint2double(a, c), __hiloint2double(b, d));
+    swap32(__double2hiint(v), a, b);
+    swap32(__double2loint(v), c, d);
+    return fmax(__hiloint2double(a, c), __hiloint2double(b, d));
+}
+// 1 / sqrt(x) to the last bits of 64: the hardware's estimate and three
+// steps of Newton's iteration.
+DEV double kv8_rsqrt(double x) {
+    double y = __builtin_amdgcn_rsq(x);
+#pragma unroll
+    for (int i = 0; i < 3; i++) y = y * (1.5 - 0.5 * x * y * y);
+    return y;
 }
 
 // The exponent of the scale for values up to `top`: the least e with
@@ -74,25 +107,23 @@ DEV uint32_t kv8_rescale4(uint32_t w, int shift) {
     return r;
 }
 
-// Rotation (and norm) of the pairs a[i], b[i] of one head's row, held by 16
+// Rotation (and norm) of the pairs a[i], b[i] of one head's row, held by LANES
 // lanes, lane j with pairs j·NP..; in 64 bits, so that the code of a value
 // next to a rounding border is that of the exact one.
-template <int NP>
+template <int NP, int LANES>
 DEV void kv8_turn(double (&a)[NP], double (&b)[NP], const cj_kv8_args &g, const float *w, int pos, int j) {
     if (g.norm) {
         double ss = 0;
 #pragma unroll
         for (int i = 0; i < NP; i++) ss += a[i] * a[i] + b[i] * b[i];
-#pragma unroll
-        for (int m = 1; m < 16; m *= 2) ss += kv8_shfl_xor(ss, m);
-        const double s = 1.0 / sqrt(ss / (32 * NP) + (double)g.eps), one = g.form ? 1.0 : 0.0;
+        const double s = kv8_rsqrt(kv8_sum<LANES>(ss) * (1.0 / (2 * LANES * NP)) + (double)g.eps), one = g.form ? 1.0 : 0.0;
 #pragma unroll
         for (int i = 0; i < NP; i++) {
             a[i] = a[i] * s * (one + (double)w[j * NP + i]);
-            b[i] = b[i] * s * (one + (double)w[16 * NP + j * NP + i]);
+            b[i] = b[i] * s * (one + (double)w[LANES * NP + j * NP + i]);
         }
     }
-    const float *cs = g.rope_cs + (int64_t)pos * (32 * NP) + 2 * NP * j;
+    const float *cs = g.rope_cs + (int64_t)pos * (2 * LANES * NP) + 2 * NP * j;
 #pragma unroll
     for (int i = 0; i < NP; i++) {
         const double c = (double)cs[2 * i], s = (double)cs[2 * i + 1], x = a[i], y = b[i];
@@ -113,35 +144,46 @@ DEV void kv8_load(const float *p, double (&a)[NP]) {
     for (int i = 0; i < NP; i++) a[i] = (double)f[i];
 }
 
+DEV void kv8_store4(float *p, const double (&a)[4]) { *(f32x4 *)p = f32x4{(float)a[0], (float)a[1], (float)a[2], (float)a[3]}; }
+
 DEV double kv8_size(double x) { return fabs(x) <= 1.0e300 ? fabs(x) : __longlong_as_double(0x7ff0000000000000ll); }
 
 DEV uint32_t kv8_code(double x, double inv) { return (uint32_t)((int)rint(x * inv) + 128); }
 
-// Append: a workgroup a (segment, block, kv head), then workgroups of 16
-// (row, query head) pairs. Thread t holds position (or pair) t / 16 and its
-// rotation pairs (t % 16)·NP.., so a head's row is 16 lanes.
+// Append: a workgroup a (segment, block, kv head), thread t position t / 16
+// of the block and its rotation pairs (t % 16)·NP.., so a head's row is 16
+// lanes; then workgroups of (row, query head) pairs, 16 bytes a lane.
 template <int HD>
 DEV void kv8_append(const cj_kv8_args &a) {
     constexpr int NP = HD / 32;
     const int t = threadIdx.x, tt = t >> 4, j = t & 15;
     Kv8Seg g;
     if ((int)blockIdx.x >= a.kv_wgs) {
-        // query rows
-        const int w = (int)blockIdx.x - a.kv_wgs, s = w / a.per_seg;
+        // query rows: KV8_QS turns of 256 / LANES (row, head) pairs, all loaded first
+        constexpr int LANES = HD / 8, PER = 256 / LANES;
+        const int w = (int)blockIdx.x - a.kv_wgs, s = w / a.per_seg, it = t / LANES, d = t % LANES * 4;
         if (!kv8_seg(a, s, g)) return;
-        const int i = (w - s * a.per_seg) * 16 + tt, r = i / a.n_q, h = i - r * a.n_q;
-        if (r >= g.rows) return;
-        double x[NP], y[NP];
-        const float *src = a.q + (int64_t)(g.row + r) * a.q_stride + (int64_t)h * HD + j * NP;
-        kv8_load<NP>(src, x);
-        kv8_load<NP>(src + HD / 2, y);
-        kv8_turn<NP>(x, y, a, a.qw, g.pos + r, j);
-        float *dst = a.q_out + (int64_t)(g.row + r) * a.out_stride + (int64_t)h * HD + j * NP;
+        double x[KV8_QS][4], y[KV8_QS][4];
+        int r[KV8_QS], h[KV8_QS];
 #pragma unroll
-        for (int i = 0; i < NP; i++) {
-            dst[i] = (float)x[i];
-            dst[HD / 2 + i] = (float)y[i];
+        for (int k = 0; k < KV8_QS; k++) {
+            const int i = ((w - s * a.per_seg) * KV8_QS + k) * PER + it;
+            r[k] = i / a.n_q;
+            h[k] = i - r[k] * a.n_q;
+            if (r[k] < g.rows) {
+                const float *src = a.q + (int64_t)(g.row + r[k]) * a.q_stride + (int64_t)h[k] * HD + d;
+                kv8_load<4>(src, x[k]);
+                kv8_load<4>(src + HD / 2, y[k]);
+            }
         }
+#pragma unroll
+        for (int k = 0; k < KV8_QS; k++)
+            if (r[k] < g.rows) {
+                kv8_turn<4, LANES>(x[k], y[k], a, a.qw, g.pos + r[k], t % LANES);
+                float *dst = a.q_out + (int64_t)(g.row + r[k]) * a.out_stride + (int64_t)h[k] * HD + d;
+                kv8_store4(dst, x[k]);
+                kv8_store4(dst + HD / 2, y[k]);
+            }
         return;
     }
     __shared__ double tops[2][4];
@@ -175,18 +217,15 @@ DEV void kv8_append(const cj_kv8_args &a) {
         kv8_load<NP>(a.k + at + HD / 2, ky);
         kv8_load<NP>(a.v + at, vx);
         kv8_load<NP>(a.v + at + HD / 2, vy);
-        kv8_turn<NP>(kx, ky, a, a.kw, p, j);
+        kv8_turn<NP, 16>(kx, ky, a, a.kw, p, j);
 #pragma unroll
         for (int i = 0; i < NP; i++) {
             ktop = fmax(ktop, fmax(kv8_size(kx[i]), kv8_size(ky[i])));
             vtop = fmax(vtop, fmax(kv8_size(vx[i]), kv8_size(vy[i])));
         }
     }
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) {
-        ktop = fmax(ktop, kv8_shfl_xor(ktop, m));
-        vtop = fmax(vtop, kv8_shfl_xor(vtop, m));
-    }
+    ktop = kv8_max64(ktop);
+    vtop = kv8_max64(vtop);
     if ((t & 63) == 0) {
         tops[0][t >> 6] = ktop;
         tops[1][t >> 6] = vtop;
@@ -320,6 +359,7 @@ DEV void kv8_read(const cj_kv8_args &a) {
 // out of f16's subnormals.
 
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -336,13 +376,36 @@ DEV h16x8 kv8_half8(uint32_t a, uint32_t b) {
     return r.h - (_Float16)1152.0f;
 }
 
+DEV uint32_t kv8_pack2(float x, float y) {
+    const f32x2 v = {x, y};
+    union { h16x2 h; uint32_t u; } r;
+    r.h = __builtin_convertvector(v, h16x2);
+    return r.u;
+}
+
+// w less its f16 half: v_fma_mix_f32 reads the half as it lies (the compiler
+// widens it first).
+DEV float kv8_less_lo(uint32_t h, float w) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(w));
+    return r;
+}
+DEV float kv8_less_hi(uint32_t h, float w) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(w));
+    return r;
+}
+
 // x as hi + lo halves.
 DEV void kv8_halves(const float (&x)[8], h16x8 &hi, h16x8 &lo) {
+    union { uint32_t u[4]; h16x8 h; } a, b;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        hi[i] = (_Float16)x[i];
-        lo[i] = (_Float16)__builtin_fmaf((float)hi[i], -1.0f, x[i]);
+    for (int i = 0; i < 4; i++) {
+        a.u[i] = kv8_pack2(x[2 * i], x[2 * i + 1]);
+        b.u[i] = kv8_pack2(kv8_less_lo(a.u[i], x[2 * i]), kv8_less_hi(a.u[i], x[2 * i + 1]));
     }
+    hi = a.h;
+    lo = b.h;
 }
 
 // The exponent of a block's scale as a float; NaN where the scale is.
@@ -352,6 +415,10 @@ DEV float kv8_recip(float s) { return __uint_as_float((254u << 23) - (__float_as
 // A column's q, an exponent k apart from [1, 2)·2^14: the factor that the
 // scores take back, scale·log2(e)·2^(k − 14).
 DEV int kv8_q_exponent(float top) { return (int)(__float_as_uint(top) >> 23) - 127; }
+
+// Keeps a branch that few pages take a branch: the compiler would carry out
+// its comparisons and selects for every page.
+DEV void kv8_branch() { asm volatile(""); }
 
 DEV float kv8_max4(float v) {   // over the lanes l, l ^ 16, l ^ 32, l ^ 48
     int a, b;
@@ -396,15 +463,15 @@ DEV float *kv8_part(const cj_kv8_args &a, int s, int h, int ct, int sp) {
 //  - output: B is the weights as they lie, A the V codes, 16 positions of a
 //    channel in 16 bytes.
 template <int HD>
-DEV void kv8_attend_few(const cj_kv8_args &a) {
+DEV void kv8_attend_c16(const cj_kv8_args &a) {
     constexpr int KS = HD / 32, DT = HD / 16, KW = HD / 64;   // steps over the channels; channel tiles; 16-byte words a lane and key
     __shared__ __align__(16) float so[4][KV8_FEW][HD + 4];
     __shared__ float sm[4][KV8_FEW], sl[4][KV8_FEW];
-    const int t = threadIdx.x, l = t & 63, wv = t >> 6, n = l & 15, g4 = l >> 4;
+    const int t = threadIdx.x, l = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), n = l & 15, g4 = l >> 4;
     // workgroups eight apart share an L2: a segment's column tiles follow one another there
-    const int64_t id = blockIdx.x, per = id / (8 * a.col_tiles), rest = per * 8 + id % 8;
-    const int ct = (int)((id / 8) % a.col_tiles);
-    const int h = (int)(rest % a.n_kv), sp = (int)((rest / a.n_kv) % a.splits), s = (int)(rest / a.n_kv / a.splits);
+    const uint32_t id = blockIdx.x, per = id / 8 / a.col_tiles, rest = per * 8 + id % 8;
+    const int ct = (int)(id / 8 % a.col_tiles);
+    const int h = (int)(rest % a.n_kv), sp = (int)(rest / a.n_kv % a.splits), s = (int)(rest / a.n_kv / a.splits);
     Kv8Seg g;
     if (s >= a.n_segs || !kv8_seg(a, s, g)) return;
     const int grp = a.n_q / a.n_kv, cols = g.rows * grp, c0 = ct * KV8_FEW;
@@ -418,32 +485,18 @@ DEV void kv8_attend_few(const cj_kv8_args &a) {
     const int c = c0 + n < cols ? c0 + n : c0, ri = c / grp;
     const int last = g.pos + ri, first = a.window > 0 ? last + 1 - a.window : 0;
     h16x8 qh[KS], ql[KS];
-    float cs;
+    float qx[KS][8], top = 0, cs;
     {
-        float x[KS][8], top = 0;
         const float *src = a.q + (int64_t)(g.row + ri) * a.q_stride + (int64_t)(h * grp + c % grp) * HD + g4 * (HD / 4);
 #pragma unroll
         for (int k = 0; k < KS; k++) {
-            *(f32x4 *)&x[k][0] = *(const f32x4 *)(src + 8 * k);
-            *(f32x4 *)&x[k][4] = *(const f32x4 *)(src + 8 * k + 4);
-#pragma unroll
-            for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[k][i]));
-        }
-        const int e = kv8_q_exponent(kv8_max4(top));
-        cs = ldexpf(a.scale * KV8_LOG2E, e - 14);
-#pragma unroll
-        for (int k = 0; k < KS; k++) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[k][i] = ldexpf(x[k][i], 14 - e);
-            kv8_halves(x[k], qh[k], ql[k]);
+            *(f32x4 *)&qx[k][0] = *(const f32x4 *)(src + 8 * k);
+            *(f32x4 *)&qx[k][4] = *(const f32x4 *)(src + 8 * k + 4);
         }
     }
-    f32x4 o[DT] = {};
-    float M = -INFINITY, L = 0;
-
     const int key0 = (n >> 2) * 16 + (n & 3);
-    u32x4 kr[4][KW], vr[DT];
-    float ks, vs;
+    u32x4 kr[4][KW], vr[DT], vn[DT];
+    float ks, vs, vsn;
     int pi = p0 + wv;
     bool bad = false;
     auto page_at = [&](int i) {
@@ -458,41 +511,68 @@ DEV void kv8_attend_few(const cj_kv8_args &a) {
 #pragma unroll
             for (int i = 0; i < KW; i++) kr[q][i] = __builtin_nontemporal_load((const u32x4 *)(b + q * 4 * HD + i * 16));
         ks = a.ks[ph * 4 + g4];
-        if (bad) ks = __uint_as_float(0x7fc00000u);
     };
     auto load_v = [&](int64_t ph) {
         const uint8_t *b = a.vc + ph * (KV8_PAGE * HD) + (g4 * HD + n) * 16;
 #pragma unroll
-        for (int j = 0; j < DT; j++) vr[j] = __builtin_nontemporal_load((const u32x4 *)(b + j * 256));
-        vs = a.vs[ph * 4 + g4];
+        for (int j = 0; j < DT; j++) vn[j] = __builtin_nontemporal_load((const u32x4 *)(b + j * 256));
+        vsn = a.vs[ph * 4 + g4];
+    };
+    auto take_v = [&]() {
+#pragma unroll
+        for (int j = 0; j < DT; j++) vr[j] = vn[j];
+        vs = vsn;
     };
     int64_t ph = 0;
     if (pi < p1) {
         ph = page_at(pi);
         load_k(ph);
         load_v(ph);
+        take_v();
     }
+    {
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(qx[k][i]));
+        const int e = kv8_q_exponent(kv8_max4(top));
+        cs = ldexpf(a.scale * KV8_LOG2E, e - 14);
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) qx[k][i] = ldexpf(qx[k][i], 14 - e);
+            kv8_halves(qx[k], qh[k], ql[k]);
+        }
+    }
+    f32x4 o[DT] = {};
+    float M = -INFINITY, L = 0;
+
     for (; pi < p1; pi += 4) {
         if (bad && a.status && l == 0) *a.status = 1;
         f32x4 x[4] = {};
 #pragma unroll
-        for (int q = 0; q < 4; q++)
+        for (int k = 0; k < KS; k++) {
+            h16x8 f[4];
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
+            for (int q = 0; q < 4; q++) {
                 const u32x4 w = kr[q][k / 2];
-                const h16x8 f = k & 1 ? kv8_half8(w[2], w[3]) : kv8_half8(w[0], w[1]);
-                x[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, qh[k], x[q], 0, 0, 0);
-                x[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, ql[k], x[q], 0, 0, 0);
+                f[q] = k & 1 ? kv8_half8(w[2], w[3]) : kv8_half8(w[0], w[1]);
+                x[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[q], qh[k], x[q], 0, 0, 0);
             }
-        const float kf = ks * cs, ve = kv8_exp_f(vs), vi = kv8_recip(vs);
+#pragma unroll
+            for (int q = 0; q < 4; q++) x[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[q], ql[k], x[q], 0, 0, 0);
+        }
+        const float kf = (bad ? __uint_as_float(0x7fc00000u) : ks) * cs, ve = kv8_exp_f(vs), vi = kv8_recip(vs);
         const bool more = pi + 4 < p1;
         if (more) {
             ph = page_at(pi + 4);
             load_k(ph);
+            load_v(ph);
         }
         float top = -INFINITY;
         const int at = pi * KV8_PAGE + g4 * 16;
         if (pi * KV8_PAGE + KV8_PAGE - 1 > g.pos + r0 || (a.window > 0 && pi * KV8_PAGE < g.pos + r1 / grp + 1 - a.window)) {
+            kv8_branch();
 #pragma unroll
             for (int q = 0; q < 4; q++)
 #pragma unroll
@@ -533,14 +613,19 @@ DEV void kv8_attend_few(const cj_kv8_args &a) {
         }
         L += sum == 0.0f ? 0.0f : sum * vi;
 #pragma unroll
-        for (int j = 0; j < DT; j++)
+        for (int u = 0; u < 2; u++)
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const h16x8 f = kv8_half8(vr[j][2 * u], vr[j][2 * u + 1]);
-                o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, wh[u], o[j], 0, 0, 0);
-                o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, wl[u], o[j], 0, 0, 0);
+            for (int j0 = 0; j0 < DT; j0 += 4) {
+                h16x8 f[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    f[j] = kv8_half8(vr[j0 + j][2 * u], vr[j0 + j][2 * u + 1]);
+                    o[j0 + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[j], wh[u], o[j0 + j], 0, 0, 0);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[j0 + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[j], wl[u], o[j0 + j], 0, 0, 0);
             }
-        if (more) load_v(ph);
+        if (more) take_v();
     }
 
     // the four waves' results as one
@@ -578,8 +663,261 @@ DEV void kv8_attend_few(const cj_kv8_args &a) {
     }
 }
 
-// Many columns (prefill chunks): a workgroup a (segment, kv head, 128 columns,
-// split), a wave 32 columns, every wave over the same pages. A page's codes
+// Scores of a page's two 32-row tiles (below): what the column at `last` does
+// not see from `first` on, at position p and after, is −inf; a block of which
+// it sees nothing may have no scale.
+DEV void kv8_mask(f32x16 (&x)[2], f32x2 &ks, f32x2 &vs, int p, int first, int last) {
+    kv8_branch();
+#pragma unroll
+    for (int q = 0; q < 2; q++, p += 16) {
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            if (p + i > last || p + i < first) x[q][i] = -INFINITY;
+        if (p > last || p + 15 < first) ks[q] = vs[q] = 1.0f;
+    }
+}
+
+// The softmax step of those tiles: the running maximum M raised, the output
+// and sum rescaled where it grew, then the weights of tile q as halves.
+template <int DT>
+struct Kv8Weights {
+    float kf[2], off[2], back[2];
+    DEV Kv8Weights(const f32x16 (&x)[2], f32x2 ks, f32x2 vs, float cs, float &M, float &L, f32x16 (&o)[DT]) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+            kf[q] = ks[q] * cs;
+            kf[q] = kf[q] < 1e-37f ? 1e-37f : kf[q];   // (never zero: −inf stays −inf)
+            off[q] = kv8_exp_f(vs[q]);
+            back[q] = kv8_recip(vs[q]);
+            float m = x[q][0];
+#pragma unroll
+            for (int i = 1; i < 16; i++) m = fmaxf(m, x[q][i]);
+            top = fmaxf(top, __builtin_fmaf(m, kf[q], off[q]));
+        }
+        int u, v;
+        swap32(__float_as_int(top), u, v);
+        const float Mn = fmaxf(M, ceilf(fmaxf(__int_as_float(u), __int_as_float(v))));
+        const float base = (Mn == -INFINITY ? 0.0f : Mn) - KV8_WEIGHT;
+        if (__any(Mn != M)) {
+            const float r = __builtin_amdgcn_exp2f(M - (base + KV8_WEIGHT));
+#pragma unroll
+            for (int j = 0; j < DT; j++) o[j] *= r;
+            L *= r;
+            M = Mn;
+        }
+        off[0] -= base;
+        off[1] -= base;
+    }
+    DEV void halves(int q, const f32x16 &x, h16x8 (&wh)[2], h16x8 (&wl)[2], float &L) const {
+        float sum = 0;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            float w[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[8 * u + i], kf[q], off[q]));
+                sum += w[i];
+            }
+            kv8_halves(w, wh[u], wl[u]);
+        }
+        L += sum == 0.0f ? 0.0f : sum * back[q];
+    }
+};
+
+// Some columns (17 and more, where 128 a workgroup would leave the chip
+// empty): as for few, every wave its own pages straight from memory, but 32
+// columns and the 32-row products. q's halves stand in LDS, being the same
+// for all waves. Tile q's row r is position 32·(r/4 % 2) + 16q + 4·(r/8) +
+// r%4, which gives lane half h = l/32 blocks 2h and 2h + 1 in order.
+#define KV8_SOME 32
+template <int HD>
+DEV void kv8_attend_c32(const cj_kv8_args &a) {
+    constexpr int KS = HD / 16, DT = HD / 32, KW = HD / 32;   // steps, channel tiles, 16-byte words a lane and key
+    constexpr int QB = 2 * KS * 64 * 16, OB = 2 * KV8_SOME * (HD + 4) * 4;
+    __shared__ __align__(16) uint8_t lds[QB > OB ? QB : OB];
+    __shared__ float sm[4][KV8_SOME], sl[4][KV8_SOME];
+    const int t = threadIdx.x, l = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), n = l & 31, hf = l >> 5;
+    const uint32_t id = blockIdx.x, per = id / 8 / a.col_tiles, rest = per * 8 + id % 8;
+    const int ct = a.col_tiles - 1 - (int)(id / 8 % a.col_tiles);
+    const int h = (int)(rest % a.n_kv), sp = (int)(rest / a.n_kv % a.splits), s = (int)(rest / a.n_kv / a.splits);
+    Kv8Seg g;
+    if (s >= a.n_segs || !kv8_seg(a, s, g)) return;
+    const int grp = a.n_q / a.n_kv, cols = g.rows * grp, c0 = ct * KV8_SOME;
+    if (c0 >= cols) return;
+    const int r0 = c0 / grp, r1 = (min(c0 + KV8_SOME, cols) - 1) / grp;
+    int p0, p1;
+    const int splits = kv8_split(a, g, r0, r1, sp, p0, p1);
+    if (sp >= splits) return;
+
+    // this lane's column (past the last: the tile's first again), and its q as halves in LDS
+    const int c = c0 + n < cols ? c0 + n : c0, ri = c / grp;
+    const int last = g.pos + ri, first = a.window > 0 ? last + 1 - a.window : 0;
+    h16x8 *qs = (h16x8 *)lds;
+    float qx[KS][8], top = 0, cs;
+    {
+        const float *src = a.q + (int64_t)(g.row + ri) * a.q_stride + (int64_t)(h * grp + c % grp) * HD + hf * (HD / 2);
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            *(f32x4 *)&qx[k][0] = *(const f32x4 *)(src + 8 * k);
+            *(f32x4 *)&qx[k][4] = *(const f32x4 *)(src + 8 * k + 4);
+        }
+    }
+    const int key0 = (n >> 2 & 1) * 32 + (n >> 3) * 4 + (n & 3);
+    u32x4 kr[2][KW], vr[2][DT];
+    f32x2 ks, vs;
+    int pi = p0 + wv;
+    bool bad = false;
+    auto page_at = [&](int i) {
+        const int p = kv8_page(a, g.slot, i);
+        bad = p < 0;
+        return (int64_t)(bad ? 0 : p) * a.n_kv + h;
+    };
+    auto load_k = [&](int64_t ph) {
+        const uint8_t *b = a.kc + ph * (KV8_PAGE * HD) + key0 * HD + hf * (HD / 2);
+#pragma unroll
+        for (int q = 0; q < 2; q++)
+#pragma unroll
+            for (int i = 0; i < KW; i++) kr[q][i] = *(const u32x4 *)(b + q * 16 * HD + i * 16);
+        ks = *(const f32x2 *)(a.ks + ph * 4 + 2 * hf);
+    };
+    auto load_v = [&](int64_t ph) {
+        const uint8_t *b = a.vc + ph * (KV8_PAGE * HD) + (2 * hf * HD + n) * 16;
+#pragma unroll
+        for (int q = 0; q < 2; q++)
+#pragma unroll
+            for (int j = 0; j < DT; j++) vr[q][j] = *(const u32x4 *)(b + (q * HD + j * 32) * 16);
+        vs = *(const f32x2 *)(a.vs + ph * 4 + 2 * hf);
+    };
+    int64_t ph = 0;
+    if (pi < p1) {
+        ph = page_at(pi);
+        load_k(ph);
+        load_v(ph);
+    }
+    {
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(qx[k][i]));
+        int u, v;
+        swap32(__float_as_int(top), u, v);
+        const int e = kv8_q_exponent(fmaxf(__int_as_float(u), __int_as_float(v)));
+        const float sign = a.scale < 0 ? -1.0f : 1.0f;
+        cs = ldexpf(a.scale * sign * KV8_LOG2E, e - 14);
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            if (k % 4 != wv) continue;   // (each wave a quarter)
+#pragma unroll
+            for (int i = 0; i < 8; i++) qx[k][i] = ldexpf(qx[k][i] * sign, 14 - e);
+            h16x8 hi, lo;
+            kv8_halves(qx[k], hi, lo);
+            qs[(2 * k) * 64 + l] = hi;
+            qs[(2 * k + 1) * 64 + l] = lo;
+        }
+    }
+    f32x16 o[DT] = {};
+    float M = -INFINITY, L = 0;
+
+    __syncthreads();
+    for (; pi < p1; pi += 4) {
+        if (bad && a.status && l == 0) *a.status = 1;
+        f32x16 x[2] = {};
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            const h16x8 qh = qs[(2 * k) * 64 + l], ql = qs[(2 * k + 1) * 64 + l];
+            h16x8 f[2];
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                const u32x4 w = kr[q][k / 2];
+                f[q] = k & 1 ? kv8_half8(w[2], w[3]) : kv8_half8(w[0], w[1]);
+                x[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[q], qh, x[q], 0, 0, 0);
+            }
+#pragma unroll
+            for (int q = 0; q < 2; q++) x[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[q], ql, x[q], 0, 0, 0);
+        }
+        f32x2 kb = ks, vb = vs;
+        if (bad) kb[0] = kb[1] = __uint_as_float(0x7fc00000u);
+        const bool more = pi + 4 < p1;
+        if (more) {
+            ph = page_at(pi + 4);
+            load_k(ph);
+        }
+        if (pi * KV8_PAGE + KV8_PAGE - 1 > g.pos + r0 || (a.window > 0 && pi * KV8_PAGE < g.pos + r1 + 1 - a.window))
+            kv8_mask(x, kb, vb, pi * KV8_PAGE + hf * 32, first, last);
+        Kv8Weights<DT> w(x, kb, vb, cs, M, L, o);
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+            h16x8 wh[2], wl[2];
+            w.halves(q, x[q], wh, wl, L);
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int j = 0; j < DT; j++) {
+                    const h16x8 f = kv8_half8(vr[q][j][2 * u], vr[q][j][2 * u + 1]);
+                    o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, wh[u], o[j], 0, 0, 0);
+                    o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, wl[u], o[j], 0, 0, 0);
+                }
+        }
+        if (more) load_v(ph);
+    }
+
+    // the four waves' results as one: rescaled to the largest maximum, then 2 and 3 onto 0 and 1, then the two
+    int u, v;
+    swap32(__float_as_int(L), u, v);
+    if (hf == 0) {
+        sm[wv][n] = M;
+        sl[wv][n] = __int_as_float(u) + __int_as_float(v);
+    }
+    __syncthreads();   // (also: q's halves are not read any more)
+    const float z = fmaxf(fmaxf(sm[0][n], sm[1][n]), fmaxf(sm[2][n], sm[3][n])), f = M == -INFINITY ? 0.0f : exp2f(M - z);
+    float (*so)[KV8_SOME][HD + 4] = (float (*)[KV8_SOME][HD + 4])lds;
+    if (wv >= 2)
+#pragma unroll
+        for (int j = 0; j < DT; j++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                f32x4 y;
+#pragma unroll
+                for (int i = 0; i < 4; i++) y[i] = o[j][4 * q + i] * f;
+                *(f32x4 *)&so[wv - 2][n][j * 32 + q * 8 + hf * 4] = y;
+            }
+    __syncthreads();
+    if (wv < 2)
+#pragma unroll
+        for (int j = 0; j < DT; j++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                f32x4 *y = (f32x4 *)&so[wv][n][j * 32 + q * 8 + hf * 4];
+                f32x4 r = *y;
+#pragma unroll
+                for (int i = 0; i < 4; i++) r[i] += o[j][4 * q + i] * f;
+                *y = r;
+            }
+    __syncthreads();
+    float *part = splits > 1 ? kv8_part<HD>(a, s, h, ct, sp) : nullptr;
+    for (int i = t; i < KV8_SOME * HD / 4; i += 256) {
+        const int k = i / (HD / 4), d = i % (HD / 4) * 4, cc = c0 + k;
+        if (cc >= cols) break;
+        const float m = fmaxf(fmaxf(sm[0][k], sm[1][k]), fmaxf(sm[2][k], sm[3][k]));
+        float b = 0;
+#pragma unroll
+        for (int w = 0; w < 4; w++) b += sm[w][k] == -INFINITY ? 0.0f : sl[w][k] * exp2f(sm[w][k] - m);
+        const f32x4 y = *(const f32x4 *)&so[0][k][d] + *(const f32x4 *)&so[1][k][d];
+        if (part) {
+            *(f32x4 *)(part + k * HD + d) = y;
+            if (d == 0) {
+                part[KV8_SOME * HD + 2 * k] = m;
+                part[KV8_SOME * HD + 2 * k + 1] = b;
+            }
+        } else {
+            *(f32x4 *)(a.out + (int64_t)(g.row + cc / grp) * a.out_stride + (int64_t)(h * grp + cc % grp) * HD + d) = y / b;
+        }
+    }
+}
+
+// Many columns (prefill chunks): a workgroup a (segment, kv head, 128
+// columns), a wave 32 columns, every wave over the same pages. A page's codes
 // become f16 once, on their way into LDS, and serve the four waves; the next
 // page's codes are on their way to registers meanwhile, so a page costs one
 // barrier. As above, the tiles' rows are placed so that lane half h = l/32
@@ -590,21 +928,20 @@ DEV void kv8_attend_few(const cj_kv8_args &a) {
 //  - V in LDS: [t][u][h][channel] words of the 8 positions 8u.. of block 2h + t.
 #define KV8_MANY 128
 template <int HD>
-DEV void kv8_attend_many(const cj_kv8_args &a) {
+DEV void kv8_attend_c128(const cj_kv8_args &a) {
     constexpr int KS = HD / 16, DT = HD / 32, CH = HD / 64;   // steps, channel tiles, 16-byte words of codes a thread and plane
     constexpr int ROW = HD * 2, BUF = KV8_PAGE * ROW;
     __shared__ __align__(16) uint8_t sk[2][BUF], sv[2][BUF];
-    const int t = threadIdx.x, l = t & 63, wv = t >> 6, n = l & 31, hf = l >> 5;
-    const int64_t id = blockIdx.x;
-    const int h = (int)(id % a.n_kv), sp = (int)(id / a.n_kv % a.splits), s = (int)(id / a.n_kv / a.splits % a.n_segs);
-    const int ct = a.col_tiles - 1 - (int)(id / a.n_kv / a.splits / a.n_segs);   // the longest first
+    const int t = threadIdx.x, l = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), n = l & 31, hf = l >> 5;
+    const uint32_t id = blockIdx.x;
+    const int h = (int)(id % a.n_kv), s = (int)(id / a.n_kv % a.n_segs);
+    const int ct = a.col_tiles - 1 - (int)(id / a.n_kv / a.n_segs);   // the longest first
     Kv8Seg g;
     if (!kv8_seg(a, s, g)) return;
     const int grp = a.n_q / a.n_kv, cols = g.rows * grp, c0 = ct * KV8_MANY;
     if (c0 >= cols) return;
     int p0, p1;
-    const int splits = kv8_split(a, g, c0 / grp, (min(c0 + KV8_MANY, cols) - 1) / grp, sp, p0, p1);
-    if (sp >= splits) return;
+    kv8_split(a, g, c0 / grp, (min(c0 + KV8_MANY, cols) - 1) / grp, 0, p0, p1);   // all of them
 
     // the wave's columns, this lane's, and its q as halves (columns past the last: the last again)
     const int w0 = min(c0 + wv * 32, cols - 1), w1 = min(c0 + wv * 32 + 31, cols - 1), c = min(c0 + wv * 32 + n, cols - 1), ri = c / grp;
@@ -653,10 +990,7 @@ DEV void kv8_attend_many(const cj_kv8_args &a) {
         }
         ksn = *(const f32x2 *)(a.ks + ph * 4 + 2 * hf);
         vsn = *(const f32x2 *)(a.vs + ph * 4 + 2 * hf);
-        if (bad) {
-            ksn[0] = ksn[1] = __uint_as_float(0x7fc00000u);
-            if (a.status && t == 0) *a.status = 1;
-        }
+        if (bad && a.status && t == 0) *a.status = 1;
     };
     auto store = [&](int b) {
 #pragma unroll
@@ -676,6 +1010,7 @@ DEV void kv8_attend_many(const cj_kv8_args &a) {
     load(p0);
     store(0);
     f32x2 ks = ksn, vs = vsn;
+    if (bad) ks[0] = ks[1] = __uint_as_float(0x7fc00000u);
     for (int pi = p0, b = 0; pi < p1; pi++, b ^= 1) {
         __syncthreads();   // the page is in buffer b; buffer b ^ 1 is free
         const bool more = pi + 1 < p1;
@@ -683,62 +1018,24 @@ DEV void kv8_attend_many(const cj_kv8_args &a) {
         if (pi * KV8_PAGE <= wlast && pi * KV8_PAGE + KV8_PAGE > wlow) {
             f32x16 x[2] = {};
 #pragma unroll
-            for (int k = 0; k < KS; k++)
+            for (int k = 0; k < KS; k++) {
+                h16x8 f[2];
 #pragma unroll
                 for (int q = 0; q < 2; q++) {
-                    const h16x8 f = *(const h16x8 *)(sk[b] + (32 * q + n) * ROW + (((2 * k + hf) ^ n) & (HD / 8 - 1)) * 16);
-                    x[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, qh[k], x[q], 0, 0, 0);
-                    x[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, ql[k], x[q], 0, 0, 0);
+                    f[q] = *(const h16x8 *)(sk[b] + (32 * q + n) * ROW + (((2 * k + hf) ^ n) & (HD / 8 - 1)) * 16);
+                    x[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[q], qh[k], x[q], 0, 0, 0);
                 }
+#pragma unroll
+                for (int q = 0; q < 2; q++) x[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[q], ql[k], x[q], 0, 0, 0);
+            }
             f32x2 kb = ks, vb = vs;
-            if (pi * KV8_PAGE + KV8_PAGE - 1 > wfirst || (a.window > 0 && pi * KV8_PAGE < wlast + 1 - a.window)) {
-#pragma unroll
-                for (int q = 0; q < 2; q++) {
-                    const int p = pi * KV8_PAGE + hf * 32 + q * 16;
-#pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        if (p + i > last || p + i < first) x[q][i] = -INFINITY;
-                    if (p > last || p + 15 < first) kb[q] = vb[q] = 1.0f;   // a block that is not seen may have no scale
-                }
-            }
-            float kf[2], ve[2], top = -INFINITY;
+            if (pi * KV8_PAGE + KV8_PAGE - 1 > wfirst || (a.window > 0 && pi * KV8_PAGE < wlast + 1 - a.window))
+                kv8_mask(x, kb, vb, pi * KV8_PAGE + hf * 32, first, last);
+            Kv8Weights<DT> sm(x, kb, vb, cs, M, L, o);
 #pragma unroll
             for (int q = 0; q < 2; q++) {
-                kf[q] = kb[q] * cs;
-                kf[q] = kf[q] < 1e-37f ? 1e-37f : kf[q];   // (never zero: -inf stays -inf)
-                ve[q] = kv8_exp_f(vb[q]);
-                float m = x[q][0];
-#pragma unroll
-                for (int i = 1; i < 16; i++) m = fmaxf(m, x[q][i]);
-                top = fmaxf(top, __builtin_fmaf(m, kf[q], ve[q]));
-            }
-            int u, v;
-            swap32(__float_as_int(top), u, v);
-            const float Mn = fmaxf(M, ceilf(fmaxf(__int_as_float(u), __int_as_float(v))));
-            const float base = (Mn == -INFINITY ? 0.0f : Mn) - KV8_WEIGHT;
-            if (__any(Mn != M)) {
-                const float r = __builtin_amdgcn_exp2f(M - (base + KV8_WEIGHT));
-#pragma unroll
-                for (int j = 0; j < DT; j++) o[j] *= r;
-                L *= r;
-                M = Mn;
-            }
-#pragma unroll
-            for (int q = 0; q < 2; q++) {
-                const float off = ve[q] - base;
                 h16x8 wh[2], wl[2];
-                float sum = 0;
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    float w[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[q][8 * u + i], kf[q], off));
-                        sum += w[i];
-                    }
-                    kv8_halves(w, wh[u], wl[u]);
-                }
-                L += sum == 0.0f ? 0.0f : sum * kv8_recip(vb[q]);
+                sm.halves(q, x[q], wh, wl, L);
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
@@ -753,90 +1050,88 @@ DEV void kv8_attend_many(const cj_kv8_args &a) {
             store(b ^ 1);
             ks = ksn;
             vs = vsn;
+            if (bad) ks[0] = ks[1] = __uint_as_float(0x7fc00000u);
         }
     }
     int u, v;
     swap32(__float_as_int(L), u, v);
     L = __int_as_float(u) + __int_as_float(v);
     if (c0 + wv * 32 + n >= cols) return;
-    float *d;
-    if (splits > 1) {
-        const int k = wv * 32 + n;
-        float *part = kv8_part<HD>(a, s, h, ct, sp);
-        if (hf == 0) {
-            part[KV8_MANY * HD + 2 * k] = M;
-            part[KV8_MANY * HD + 2 * k + 1] = L;
-        }
-        d = part + k * HD;
-        L = 1.0f;
-    } else {
-        d = a.out + (int64_t)(g.row + ri) * a.out_stride + (int64_t)(h * grp + c % grp) * HD;
-    }
+    L = 1.0f / L;
+    float *d = a.out + (int64_t)(g.row + ri) * a.out_stride + (int64_t)(h * grp + c % grp) * HD;
 #pragma unroll
     for (int j = 0; j < DT; j++)
 #pragma unroll
         for (int q = 0; q < 4; q++) {
             f32x4 y;
 #pragma unroll
-            for (int i = 0; i < 4; i++) y[i] = o[j][4 * q + i] / L;
+            for (int i = 0; i < 4; i++) y[i] = o[j][4 * q + i] * L;
             *(f32x4 *)(d + j * 32 + q * 8 + hf * 4) = y;
         }
 }
 
-// The splits of a column as one row: a workgroup a (segment, kv head, column),
-// 256 / HD threads a channel over the splits in turn, joined in order.
+// The splits of the columns as one row each: HD / 4 threads a channel group,
+// a.join_ways of them side by side over a column's splits, which are then
+// joined in order; the other threads of the workgroup are other columns.
 template <int HD>
 DEV void kv8_join(const cj_kv8_args &a) {
-    constexpr int W = 256 / (HD / 4);
+    constexpr int C4 = HD / 4, W = 256 / C4;
     __shared__ __align__(16) float so[W][HD];
     __shared__ float sm[W], sl[W];
-    const int t = threadIdx.x, d = t % (HD / 4) * 4, w = t / (HD / 4);
-    const int grp = a.n_q / a.n_kv, most = a.max_rows * grp;
-    const int c = blockIdx.x % most, h = blockIdx.x / most % a.n_kv, s = blockIdx.x / most / a.n_kv;
+    const int t = threadIdx.x, d = t % C4 * 4, w = t / C4, ways = a.join_ways, per = W / ways, way = w % ways;
+    const int grp = a.n_q / a.n_kv, most = a.max_rows * grp, tiles = (most + per - 1) / per;
+    const int h = blockIdx.x / tiles % a.n_kv, s = blockIdx.x / tiles / a.n_kv, c = blockIdx.x % tiles * per + w / ways;
     Kv8Seg g;
-    if (!kv8_seg(a, s, g) || c >= g.rows * grp) return;
-    const int tc = a.tile_cols, ct = c / tc, k = c % tc, c0 = ct * tc;
-    int p0, p1;
-    const int splits = kv8_split(a, g, c0 / grp, (min(c0 + tc, g.rows * grp) - 1) / grp, 0, p0, p1);
-    if (splits <= 1) return;
-    const float *part = kv8_part<HD>(a, s, h, ct, 0);
+    if (!kv8_seg(a, s, g)) return;
+    const int cols = g.rows * grp, tc = a.tile_cols, ct = c / tc, k = c - ct * tc, c0 = ct * tc;
+    int p0, p1, splits = 0;
+    if (c < cols) splits = kv8_split(a, g, c0 / grp, (min(c0 + tc, cols) - 1) / grp, 0, p0, p1);
     float M = -INFINITY, L = 0;
     f32x4 y = {};
-    for (int sp = w; sp < splits; sp += W) {
-        const float *p = part + (int64_t)sp * (tc * (HD + 2));
-        const float m = p[tc * HD + 2 * k], b = p[tc * HD + 2 * k + 1];
-        const f32x4 v = *(const f32x4 *)(p + k * HD + d);
-        const float Mn = fmaxf(M, m), z = Mn == -INFINITY ? 0.0f : Mn, f0 = exp2f(M - z), f1 = exp2f(m - z);
-        y = y * f0 + v * f1;
-        L = L * f0 + b * f1;
-        M = Mn;
+    if (splits > 1) {
+        const float *part = kv8_part<HD>(a, s, h, ct, 0);
+        const int64_t step = (int64_t)tc * (HD + 2);
+#pragma unroll 4
+        for (int sp = way; sp < splits; sp += ways) {
+            const float *p = part + sp * step;
+            const float m = p[tc * HD + 2 * k], b = p[tc * HD + 2 * k + 1];
+            const f32x4 v = *(const f32x4 *)(p + k * HD + d);
+            const float Mn = fmaxf(M, m), z = Mn == -INFINITY ? 0.0f : Mn, f0 = exp2f(M - z), f1 = exp2f(m - z);
+            y = y * f0 + v * f1;
+            L = L * f0 + b * f1;
+            M = Mn;
+        }
     }
-    *(f32x4 *)&so[w][d] = y;
-    if (d == 0) {
-        sm[w] = M;
-        sl[w] = L;
+    if (ways > 1) {
+        *(f32x4 *)&so[w][d] = y;
+        if (d == 0) {
+            sm[w] = M;
+            sl[w] = L;
+        }
+        __syncthreads();
+        if (way) return;
+        for (int i = 1; i < ways; i++) M = fmaxf(M, sm[w + i]);
+        const float z = M == -INFINITY ? 0.0f : M;
+        y = f32x4{};
+        L = 0;
+        for (int i = 0; i < ways; i++) {
+            const float f = exp2f(sm[w + i] - z);
+            y += *(const f32x4 *)&so[w + i][d] * f;
+            L += sl[w + i] * f;
+        }
     }
-    __syncthreads();
-    if (w) return;
-    for (int i = 1; i < W; i++) M = fmaxf(M, sm[i]);
-    const float z = M == -INFINITY ? 0.0f : M;
-    f32x4 r = {};
-    float b = 0;
-    for (int i = 0; i < W; i++) {
-        const float f = exp2f(sm[i] - z);
-        r += *(const f32x4 *)&so[i][d] * f;
-        b += sl[i] * f;
-    }
-    *(f32x4 *)(a.out + (int64_t)(g.row + c / grp) * a.out_stride + (int64_t)(h * grp + c % grp) * HD + d) = r / b;
+    if (splits > 1) *(f32x4 *)(a.out + (int64_t)(g.row + c / grp) * a.out_stride + (int64_t)(h * grp + c % grp) * HD + d) = y / L;
 }
 
 extern "C" __global__ void __launch_bounds__(256) cj_kv8_append_h64(cj_kv8_args a) { kv8_append<64>(a); }
 extern "C" __global__ void __launch_bounds__(256) cj_kv8_append_h128(cj_kv8_args a) { kv8_append<128>(a); }
 extern "C" __global__ void __launch_bounds__(256) cj_kv8_read_h64(cj_kv8_args a) { kv8_read<64>(a); }
 extern "C" __global__ void __launch_bounds__(256) cj_kv8_read_h128(cj_kv8_args a) { kv8_read<128>(a); }
-extern "C" __global__ void __launch_bounds__(256, 2) cj_kv8_attend_few_h64(cj_kv8_args a) { kv8_attend_few<64>(a); }
-extern "C" __global__ void __launch_bounds__(256, 2) cj_kv8_attend_few_h128(cj_kv8_args a) { kv8_attend_few<128>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) cj_kv8_attend_c16_h64(cj_kv8_args a) { kv8_attend_c16<64>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) cj_kv8_attend_c16_h128(cj_kv8_args a) { kv8_attend_c16<128>(a); }
 extern "C" __global__ void __launch_bounds__(256) cj_kv8_join_h64(cj_kv8_args a) { kv8_join<64>(a); }
 extern "C" __global__ void __launch_bounds__(256) cj_kv8_join_h128(cj_kv8_args a) { kv8_join<128>(a); }
-extern "C" __global__ void __launch_bounds__(256, 2) cj_kv8_attend_many_h64(cj_kv8_args a) { kv8_attend_many<64>(a); }
-extern "C" __global__ void __launch_bounds__(256, 2) cj_kv8_attend_many_h128(cj_kv8_args a) { kv8_attend_many<128>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) cj_kv8_attend_c32_h64(cj_kv8_args a) { kv8_attend_c32<64>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) cj_kv8_attend_c32_h128(cj_kv8_args a) { kv8_attend_c32<128>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) cj_kv8_attend_c128_h64(cj_kv8_args a) { kv8_attend_c128<64>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) cj_kv8_attend_c128_h128(cj_kv8_args a) { kv8_attend_c128<128>(a); }

@@ -57,23 +57,32 @@ int run(const char *kernel, int32_t hd, int64_t grid, uint32_t block, const cj_k
     return launch((std::string(kernel) + "_h" + std::to_string(hd)).c_str(), (uint32_t)grid, block, 0, a);
 }
 
-// How a call runs: the column tiles of a segment (a column is a row and a
-// query head of one kv head's group), and the positions' split over enough
-// workgroups to fill the chip.
+// How a call runs. A column is a row and a query head of one kv head's group;
+// a workgroup takes 16, 32 or 128 of a segment's and, up to 32, a part of the
+// positions (a wave a page at a time), whose parts a second launch joins.
+// Measured on 256 CUs at head size 128, 4 heads a kv head, 8 kv heads:
+//  - 128 columns a workgroup convert a page once for four waves, but keep a
+//    chip of 256 CUs busy only where there are enough of them (us, 32 → 128;
+//    1024 rows behind 1033, 256 workgroups of 128: 77 → 80; 1536 rows, 384:
+//    121 → 114; 2048 rows, 512: 171 → 150);
+//  - the positions are split for two workgroups a CU, what fits one (one
+//    sequence of 65500: 32.7 us, for one 35.4, three 36.6, six 41.6; 32
+//    sequences of 16384: 177, 196, 182, 183), and not where it saves a wave
+//    two pages or less, about 2 us each, for the join's 4 us (32 sequences of
+//    1024, a split or none: 23.6 and 17.6; one of 257: 10.9 and 8.3).
 struct Plan {
-    bool many;
     int64_t tile_cols, col_tiles, splits, split_pages, bytes;
 };
 Plan plan_attend(int64_t n_segs, int64_t max_rows, int64_t max_count, int64_t n_q, int64_t n_kv, int64_t hd, int64_t window) {
     Plan p;
-    const int64_t cols = max_rows * (n_q / n_kv), cus = std::max(1, device_cus());
-    p.many = cols > 64;
-    p.tile_cols = p.many ? 128 : 16;
+    const int64_t cols = max_rows * (n_q / n_kv), cus = std::max(1, device_cus()), heads = n_segs * n_kv;
+    p.tile_cols = cols <= 16 ? 16 : 4 * heads * ((cols + 127) / 128) < 5 * cus ? 32 : 128;
     p.col_tiles = (cols + p.tile_cols - 1) / p.tile_cols;
     int64_t pages = (max_count + 63) / 64;
-    if (window) pages = std::min(pages, (window + max_rows) / 64 + 2);   // what the rows of a tile see together
-    const int64_t units = n_segs * n_kv * p.col_tiles, want = std::max<int64_t>(1, (p.many ? 2 : 3) * cus / units);
+    if (window) pages = std::min(pages, (window + max_rows) / 64 + 2);   // what a tile's rows see together
+    const int64_t units = heads * p.col_tiles, want = std::max<int64_t>(1, 2 * cus / units);
     p.split_pages = std::max<int64_t>(4, (pages + want - 1) / want);
+    if (p.tile_cols == 128 || pages <= p.split_pages + 8) p.split_pages = pages;
     p.splits = (pages + p.split_pages - 1) / p.split_pages;
     p.bytes = p.splits > 1 ? units * p.splits * p.tile_cols * (hd + 2) * 4 : 0;
     return p;
@@ -115,7 +124,7 @@ int32_t cj_kv8_append(int64_t q_out, int64_t q, int64_t k, int64_t v, int64_t kp
     a.q_stride = q_stride; a.kv_stride = kv_stride; a.out_stride = q_out_stride;
     a.limit = std::min(a.limit, rope_ctx);
     a.norm = norm != 0; a.form = form; a.eps = eps;
-    const int64_t kv = blocks_of(max_rows) * n_segs * n_kv, per = q ? ((int64_t)max_rows * n_q + 15) / 16 : 0;
+    const int64_t kv = blocks_of(max_rows) * n_segs * n_kv, items = KV8_QS * 2048 / head_dim, per = q ? ((int64_t)max_rows * n_q + items - 1) / items : 0;
     if (kv > 0x7fffffff || per > 0x7fffffff) return fail(CJ_ERR_ARG, "cj_kv8_append: %d x %d rows exceed a launch", n_segs, max_rows);
     a.kv_wgs = (int32_t)kv; a.per_seg = (int32_t)per;
     return run("cj_kv8_append", head_dim, kv + per * n_segs, 256, a);
@@ -161,13 +170,16 @@ int32_t cj_kv8_attend(int64_t out, int64_t q, int64_t kplane, int64_t vplane, in
     const Plan p = plan_attend(n_segs, max_rows, max_count, n_q, n_kv, head_dim, window);
     if (p.bytes && ((part & 15) || !in_buffer(dptr(part), p.bytes)))
         return fail(CJ_ERR_ARG, "cj_kv8_attend: part is not 16-byte aligned or smaller than %lld bytes", (long long)p.bytes);
-    const int64_t units = (int64_t)n_segs * n_kv * p.splits, join = (int64_t)n_segs * max_rows * n_q;
-    const int64_t wgs = (p.many ? units : (units + 7) / 8 * 8) * p.col_tiles;
+    // the join: as many threads over a column's splits as there are splits, of the W that a workgroup has for its columns
+    int64_t ways = 1, W = 1024 / head_dim;
+    while (ways < W && ways < p.splits) ways *= 2;
+    const int64_t units = (int64_t)n_segs * n_kv * p.splits, per = W / ways, cols = (int64_t)max_rows * (n_q / n_kv);
+    const int64_t wgs = (p.tile_cols == 128 ? units : (units + 7) / 8 * 8) * p.col_tiles, join = (int64_t)n_segs * n_kv * ((cols + per - 1) / per);
     if (wgs > 0x7fffffff || join > 0x7fffffff)
         return fail(CJ_ERR_ARG, "cj_kv8_attend: %d x %d rows of %d heads exceed a launch", n_segs, max_rows, n_q);
-    a.part = (float *)dptr(part); a.col_tiles = (int32_t)p.col_tiles; a.tile_cols = (int32_t)p.tile_cols; a.splits = (int32_t)p.splits;
-    a.split_pages = (int32_t)p.split_pages;
-    const int rc = run(p.many ? "cj_kv8_attend_many" : "cj_kv8_attend_few", head_dim, wgs, 256, a);
+    a.part = (float *)dptr(part); a.col_tiles = (int32_t)p.col_tiles; a.tile_cols = (int32_t)p.tile_cols;
+    a.splits = (int32_t)p.splits; a.split_pages = (int32_t)p.split_pages; a.join_ways = (int32_t)ways;
+    const int rc = run(p.tile_cols == 16 ? "cj_kv8_attend_c16" : p.tile_cols == 32 ? "cj_kv8_attend_c32" : "cj_kv8_attend_c128", head_dim, wgs, 256, a);
     return rc || p.splits == 1 ? rc : run("cj_kv8_join", head_dim, join, 256, a);
 }
 

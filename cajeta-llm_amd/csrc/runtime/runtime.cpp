@@ -535,8 +535,8 @@ int32_t cj_init(int32_t device) {
         "cj_attn_scores_rows_f32_h64", "cj_attn_scores_rows_f32_h128", "cj_attn_combine_rows_f32_h64",
         "cj_attn_combine_rows_f32_h128",
         "cj_kv8_append_h64", "cj_kv8_append_h128", "cj_kv8_read_h64", "cj_kv8_read_h128",
-        "cj_kv8_attend_few_h64", "cj_kv8_attend_few_h128", "cj_kv8_attend_many_h64",
-        "cj_kv8_attend_many_h128", "cj_kv8_join_h64", "cj_kv8_join_h128",
+        "cj_kv8_attend_c16_h64", "cj_kv8_attend_c16_h128", "cj_kv8_attend_c32_h64", "cj_kv8_attend_c32_h128",
+        "cj_kv8_attend_c128_h64", "cj_kv8_attend_c128_h128", "cj_kv8_join_h64", "cj_kv8_join_h128",
     };
     for (const char *k : kernels) {
         hipFunction_t f;

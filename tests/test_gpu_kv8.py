@@ -322,6 +322,21 @@ def test_pages_outside_the_pool_are_not_touched(gpu, page):
 COUNTS = [1, 2, 15, 16, 17, 63, 64, 65, 127, 200, 449, 1030]
 
 
+@pytest.mark.parametrize("rows,heads,kv,count,names", [
+    (1, 32, 8, 64, ["c16"]), (1, 32, 8, 512, ["c16"]), (1, 32, 8, 2049, ["c16", "join"]), (1, 40, 2, 64, ["c32"]),
+    (6, 32, 8, 2049, ["c32", "join"]), (300, 32, 8, 300, ["c32"])])
+def test_which_kernels_run(gpu, launched, rows, heads, kv, count, names):
+    """Few and many columns, with and without a split, alone and in both head sizes (128 columns: below)."""
+    rng = np.random.default_rng(rows + count)
+    for hd in (64, 128):
+        P = Pages(gpu, heads, kv, hd, 1, 33, seed=rows)
+        P.append([(0, 0, 0, count)], *rows_of(rng, count, heads, kv, hd))
+        q = rows_of(rng, rows, heads, kv, hd)[0]
+        got, seen = launched(lambda: P.check_attend([(0, count - rows, 0, rows)], q))
+        assert seen == ["cj_kv8_%s_h%d" % ("join" if n == "join" else "attend_" + n, hd) for n in names]
+        assert np.array_equal(got, P.check_attend([(0, count - rows, 0, rows)], q))
+
+
 @pytest.mark.parametrize("window", [0, 1, 40])
 @pytest.mark.parametrize("heads,kv,hd", [(8, 2, 64), (32, 8, 128), (2, 2, 128), (16, 1, 64), (24, 1, 128), (64, 1, 64)])
 def test_attention_of_one_row(gpu, heads, kv, hd, window):
@@ -367,6 +382,46 @@ def test_attention_of_chunks(gpu, heads, kv, hd, window):
     P.check_attend([(0, 0, 0, 211), (1, 450, 211, 62), (2, 0, 273, 64), (3, 1, 337, 128)], q, window)
     P.check_attend([(1, 385, 0, 127)], q[:127], window)
     assert P.stat() == 0
+
+
+@pytest.mark.parametrize("window", [0, 37])
+@pytest.mark.parametrize("heads,kv,hd,n", [(32, 8, 128, 44), (8, 8, 64, 44), (30, 6, 128, 56)])
+def test_attention_of_chunks_that_fill_the_chip(gpu, launched, heads, kv, hd, n, window):
+    """Enough segments of enough rows for the 128-column workgroups; ragged, from inside pages, some of one row or none."""
+    say("kv8 many", heads, kv, hd, window)
+    rng = np.random.default_rng(heads + hd + window)
+    rows = rng.integers(17, 34, n) * (4 if heads == kv else 1)
+    rows[3], rows[5], rows[7] = 0, 1, rows.max()
+    before = rng.integers(0, 90, n)
+    before[:8] = (0, 64, 63, 5, 1, 100, 47, 48)
+    slots = rng.permutation(n)
+    P = Pages(gpu, heads, kv, hd, n, 4, seed=window)
+    at = np.cumsum(np.concatenate(([0], before + rows)))
+    P.append([(int(s), 0, int(a), int(b + r)) for s, a, b, r in zip(slots, at, before, rows)],
+             *rows_of(rng, int(at[-1]), heads, kv, hd))
+    at = np.cumsum(np.concatenate(([2], rows)))
+    q = rows_of(rng, int(at[-1]) + 2, heads, kv, hd)[0] * np.float32(2)
+    segs = [(int(s), int(b), int(a), int(r)) for s, a, b, r in zip(slots, at, before, rows)]
+    got, names = launched(lambda: P.check_attend(segs, q, window))
+    assert names == ["cj_kv8_attend_c128_h%d" % hd]
+    assert np.array_equal(got, P.check_attend(segs, q, window))      # and the same again
+    q[at[5], 0, 3] = np.nan
+    bad, _ = P.attend(segs, q, window)
+    same = np.isnan(bad[at[5], 0]).all() and np.array_equal(bad[at[5], 1:], got[at[5], 1:])
+    assert same and np.array_equal(np.delete(bad, at[5], 0), np.delete(got, at[5], 0))
+    assert P.stat() == 0
+    # a page outside the pool: its rows are NaN, the others stay
+    k = 7
+    P.table[slots[k], 0] = P.pool
+    P.tab.upload(P.table)
+    q[at[5], 0, 3] = 1.0
+    bad, _ = P.attend(segs, q, window)
+    assert P.stat() == 1
+    mine = slice(int(at[k]), int(at[k] + rows[k]))
+    last = before[k] + np.arange(rows[k])
+    first = np.maximum(0, last + 1 - window) if window else np.zeros_like(last)
+    assert np.array_equal(np.isnan(bad[mine]).all((1, 2)), first < PAGE)
+    assert np.isfinite(np.delete(bad, np.r_[mine], 0)).all()
 
 
 def test_loud_and_quiet_blocks_and_far_scores(gpu):
