@@ -453,6 +453,85 @@ DEV float *kv8_part(const cj_kv8_args &a, int s, int h, int ct, int sp) {
     return a.part + ((((int64_t)s * a.n_kv + h) * a.col_tiles + ct) * a.splits + sp) * (a.tile_cols * (HD + 2));
 }
 
+// Page ids of a run of pages, 64 at a time, one a lane: read where a page is
+// loaded, each would cost the wave a round trip to memory.
+struct Kv8Table {
+    const cj_kv8_args &a;
+    const int slot, from, step, end;   // pages from, from + step, .. before end
+    int ids;
+    // the id of page from + step·k (k from 0 up, one after the other), −1 where there is none
+    DEV int at(int k) {
+        if ((k & 63) == 0) ids = kv8_page(a, slot, min(end - 1, from + step * (k + (int)(threadIdx.x & 63))));
+        return __builtin_amdgcn_readlane(ids, k & 63);
+    }
+};
+
+// A page's K codes go from memory straight into the wave's part of LDS, eight
+// (HD 128) or four lanes a row, so that a copy touches whole lines (a lane a
+// row, 64 lines an instruction, cost the c32 kernel more than its products).
+// LDS row ρ holds key `key(ρ)` of the page; its 16-byte word c stands at c ^
+// swizzle(ρ), so that eight rows' reads of one word fall on all banks once.
+template <int HD>
+DEV int kv8_swizzle(int row) { return HD == 128 ? row & 7 : row >> 2 & 3; }
+template <int HD, class Key>
+DEV void kv8_copy_k(const uint8_t *page, uint8_t *lds, int l, Key &&key) {
+    constexpr int W = HD / 16;   // words a row
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the page that stood there has been read
+#pragma unroll
+    for (int e = 0; e < W; e++) {
+        const int row = e * (64 / W) + l / W, c = l % W ^ kv8_swizzle<HD>(row);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(page + key(row) * HD + c * 16),
+                                         (__attribute__((address_space(3))) void *)(lds + e * 1024), 16, 0, 0);
+    }
+}
+template <int HD>
+DEV u32x4 kv8_read_k(const uint8_t *lds, int row, int c) {
+    return *(const u32x4 *)(lds + row * HD + (c ^ kv8_swizzle<HD>(row)) * 16);
+}
+// The wave's copies and loads have landed.
+DEV void kv8_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// The columns' q as halves into LDS in the products' operand order: C columns
+// of 256 / C threads, thread j of column c with its channels 4j + i·1024/C..;
+// `at(d)` is the operand word and lane part of channel d. cs[c] takes back the
+// column's exponent: scale·log2(e)·2^(k − 14), for the largest in [1, 2)·2^k.
+template <int HD, int C>
+struct Kv8Q {
+    static constexpr int T = 256 / C, N = HD / (4 * T);
+    f32x4 x[N];
+    DEV void load(const float *src, int j) {
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = *(const f32x4 *)(src + i * 4 * T + j * 4);
+    }
+    template <class At>
+    DEV void store(uint8_t *qs, float *cs, int c, int j, float scale, At &&at) const {
+        float top = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) top = fmaxf(top, fabsf(x[i][k]));
+        top = fmaxf(top, dpp_f<DPP_XOR1>(top));
+        top = fmaxf(top, dpp_f<DPP_XOR2>(top));
+        top = fmaxf(top, dpp_f<DPP_HMIRROR>(top));
+        if (T == 16) top = fmaxf(top, dpp_f<KV8_MIRROR>(top));
+        const int e = kv8_q_exponent(top);
+        const float sign = scale < 0 ? -1.0f : 1.0f;
+        if (j == 0) cs[c] = ldexpf(scale * sign * KV8_LOG2E, e - 14);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            float y[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) y[k] = ldexpf(x[i][k] * sign, 14 - e);
+            const uint32_t h0 = kv8_pack2(y[0], y[1]), h1 = kv8_pack2(y[2], y[3]);
+            const uint32_t l0 = kv8_pack2(kv8_less_lo(h0, y[0]), kv8_less_hi(h0, y[1]));
+            const uint32_t l1 = kv8_pack2(kv8_less_lo(h1, y[2]), kv8_less_hi(h1, y[3]));
+            uint8_t *d = qs + at(i * 4 * T + j * 4);
+            *(uint2 *)d = make_uint2(h0, h1);
+            *(uint2 *)(d + 1024) = make_uint2(l0, l1);
+        }
+    }
+};
+
 // Few columns (a column is a row and one query head of the kv head's group):
 // a workgroup a (segment, kv head, 16 columns, split), its four waves a page
 // each in turn. All operands come straight from memory to registers, in the
@@ -464,114 +543,105 @@ DEV float *kv8_part(const cj_kv8_args &a, int s, int h, int ct, int sp) {
 //    channel in 16 bytes.
 template <int HD>
 DEV void kv8_attend_c16(const cj_kv8_args &a) {
-    constexpr int KS = HD / 32, DT = HD / 16, KW = HD / 64;   // steps over the channels; channel tiles; 16-byte words a lane and key
-    __shared__ __align__(16) float so[4][KV8_FEW][HD + 4];
-    __shared__ float sm[4][KV8_FEW], sl[4][KV8_FEW];
+    constexpr int KS = HD / 32, DT = HD / 16;   // steps over the channels; channel tiles
+    constexpr int KB = KV8_PAGE * HD, OB = 4 * KV8_FEW * (HD + 4) * 4;
+    __shared__ __align__(16) uint8_t lds[4 * KB > OB ? 4 * KB : OB], qs[2 * KS * 1024];
+    __shared__ float sc[KV8_FEW], sm[4][KV8_FEW], sl[4][KV8_FEW];
     const int t = threadIdx.x, l = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), n = l & 15, g4 = l >> 4;
-    // workgroups eight apart share an L2: a segment's column tiles follow one another there
-    const uint32_t id = blockIdx.x, per = id / 8 / a.col_tiles, rest = per * 8 + id % 8;
-    const int ct = (int)(id / 8 % a.col_tiles);
-    const int h = (int)(rest % a.n_kv), sp = (int)(rest / a.n_kv % a.splits), s = (int)(rest / a.n_kv / a.splits);
+    const uint32_t id = blockIdx.x;
+    const int h = (int)(id % a.n_kv), sp = (int)(id / a.n_kv % a.splits), s = (int)(id / a.n_kv / a.splits);
     Kv8Seg g;
-    if (s >= a.n_segs || !kv8_seg(a, s, g)) return;
-    const int grp = a.n_q / a.n_kv, cols = g.rows * grp, c0 = ct * KV8_FEW;
-    if (c0 >= cols) return;
-    const int r0 = c0 / grp, r1 = min(c0 + KV8_FEW, cols) - 1;   // (r1: a column here)
+    if (!kv8_seg(a, s, g)) return;
+    const int grp = a.n_q / a.n_kv, cols = g.rows * grp;
+    if (cols == 0) return;
     int p0, p1;
-    const int splits = kv8_split(a, g, r0, r1 / grp, sp, p0, p1);
+    const int splits = kv8_split(a, g, 0, g.rows - 1, sp, p0, p1);
     if (sp >= splits) return;
 
-    // this lane's column (past the last: the tile's first again), and its q as halves
-    const int c = c0 + n < cols ? c0 + n : c0, ri = c / grp;
-    const int last = g.pos + ri, first = a.window > 0 ? last + 1 - a.window : 0;
-    h16x8 qh[KS], ql[KS];
-    float qx[KS][8], top = 0, cs;
+    // q of column t / 16 (past the last: the first again)
+    Kv8Q<HD, KV8_FEW> q;
     {
-        const float *src = a.q + (int64_t)(g.row + ri) * a.q_stride + (int64_t)(h * grp + c % grp) * HD + g4 * (HD / 4);
-#pragma unroll
-        for (int k = 0; k < KS; k++) {
-            *(f32x4 *)&qx[k][0] = *(const f32x4 *)(src + 8 * k);
-            *(f32x4 *)&qx[k][4] = *(const f32x4 *)(src + 8 * k + 4);
-        }
+        const int c = t / 16 < cols ? t / 16 : 0;
+        q.load(a.q + (int64_t)(g.row + c / grp) * a.q_stride + (int64_t)(h * grp + c % grp) * HD, t % 16);
     }
-    const int key0 = (n >> 2) * 16 + (n & 3);
-    u32x4 kr[4][KW], vr[DT], vn[DT];
-    float ks, vs, vsn;
+    uint8_t *kl = lds + wv * KB;
+    u32x4 vr[DT], vn[DT];
+    float ks, vs;
     int pi = p0 + wv;
+    Kv8Table table{a, g.slot, pi, 4, p1, 0};
     bool bad = false;
+    int64_t ph = 0;
     auto page_at = [&](int i) {
-        const int p = kv8_page(a, g.slot, i);
+        const int p = table.at((i - p0) >> 2);
         bad = p < 0;
-        return (int64_t)(bad ? 0 : p) * a.n_kv + h;
+        ph = (int64_t)(bad ? 0 : p) * a.n_kv + h;
     };
-    auto load_k = [&](int64_t ph) {
-        const uint8_t *b = a.kc + ph * (KV8_PAGE * HD) + key0 * HD + g4 * (HD / 4);
-#pragma unroll
-        for (int q = 0; q < 4; q++)
-#pragma unroll
-            for (int i = 0; i < KW; i++) kr[q][i] = __builtin_nontemporal_load((const u32x4 *)(b + q * 4 * HD + i * 16));
+    auto copy_k = [&]() {
+        kv8_copy_k<HD>(a.kc + ph * KB, kl, l, [](int row) { return (row >> 2 & 3) * 16 + (row >> 4) * 4 + (row & 3); });
+    };
+    auto load_v = [&]() {
         ks = a.ks[ph * 4 + g4];
-    };
-    auto load_v = [&](int64_t ph) {
-        const uint8_t *b = a.vc + ph * (KV8_PAGE * HD) + (g4 * HD + n) * 16;
+        vs = a.vs[ph * 4 + g4];
+        const uint8_t *b = a.vc + ph * KB + (g4 * HD + n) * 16;
 #pragma unroll
         for (int j = 0; j < DT; j++) vn[j] = __builtin_nontemporal_load((const u32x4 *)(b + j * 256));
-        vsn = a.vs[ph * 4 + g4];
     };
-    auto take_v = [&]() {
-#pragma unroll
-        for (int j = 0; j < DT; j++) vr[j] = vn[j];
-        vs = vsn;
-    };
-    int64_t ph = 0;
     if (pi < p1) {
-        ph = page_at(pi);
-        load_k(ph);
-        load_v(ph);
-        take_v();
+        page_at(pi);
+        copy_k();
+        load_v();
     }
-    {
+    q.store(qs, sc, t / 16, t % 16, a.scale, [t](int d) {
+        return (d % (HD / 4) / 8) * 2048 + (d / (HD / 4) * 16 + t / 16) * 16 + d % 8 * 2;
+    });
+    lds_barrier();
+    const int c = n < cols ? n : 0, last = g.pos + c / grp, first = a.window > 0 ? last + 1 - a.window : 0;
+    const float cs = sc[n];
+    h16x8 qh[KS], ql[KS];
 #pragma unroll
-        for (int k = 0; k < KS; k++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(qx[k][i]));
-        const int e = kv8_q_exponent(kv8_max4(top));
-        cs = ldexpf(a.scale * KV8_LOG2E, e - 14);
-#pragma unroll
-        for (int k = 0; k < KS; k++) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) qx[k][i] = ldexpf(qx[k][i], 14 - e);
-            kv8_halves(qx[k], qh[k], ql[k]);
-        }
+    for (int k = 0; k < KS; k++) {
+        qh[k] = *(const h16x8 *)(qs + k * 2048 + l * 16);
+        ql[k] = *(const h16x8 *)(qs + k * 2048 + 1024 + l * 16);
     }
     f32x4 o[DT] = {};
     float M = -INFINITY, L = 0;
-
     for (; pi < p1; pi += 4) {
+        kv8_landed();
         if (bad && a.status && l == 0) *a.status = 1;
+        float kf = (bad ? __uint_as_float(0x7fc00000u) : ks) * cs;
+        const float ve = kv8_exp_f(vs), vi = kv8_recip(vs);
+#pragma unroll
+        for (int j = 0; j < DT; j++) vr[j] = vn[j];
+        const bool more = pi + 4 < p1;
+        if (more) {
+            page_at(pi + 4);
+            load_v();
+        }
         f32x4 x[4] = {};
 #pragma unroll
-        for (int k = 0; k < KS; k++) {
+        for (int k = 0; k < KS; k += 2) {
+            u32x4 w[4];
             h16x8 f[4];
 #pragma unroll
             for (int q = 0; q < 4; q++) {
-                const u32x4 w = kr[q][k / 2];
-                f[q] = k & 1 ? kv8_half8(w[2], w[3]) : kv8_half8(w[0], w[1]);
+                w[q] = kv8_read_k<HD>(kl, q * 16 + n, g4 * (HD / 64) + k / 2);
+                f[q] = kv8_half8(w[q][0], w[q][1]);
                 x[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[q], qh[k], x[q], 0, 0, 0);
             }
 #pragma unroll
             for (int q = 0; q < 4; q++) x[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[q], ql[k], x[q], 0, 0, 0);
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                f[q] = kv8_half8(w[q][2], w[q][3]);
+                x[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[q], qh[k + 1], x[q], 0, 0, 0);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; q++) x[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[q], ql[k + 1], x[q], 0, 0, 0);
         }
-        const float kf = (bad ? __uint_as_float(0x7fc00000u) : ks) * cs, ve = kv8_exp_f(vs), vi = kv8_recip(vs);
-        const bool more = pi + 4 < p1;
-        if (more) {
-            ph = page_at(pi + 4);
-            load_k(ph);
-            load_v(ph);
-        }
+        if (more) copy_k();
         float top = -INFINITY;
         const int at = pi * KV8_PAGE + g4 * 16;
-        if (pi * KV8_PAGE + KV8_PAGE - 1 > g.pos + r0 || (a.window > 0 && pi * KV8_PAGE < g.pos + r1 / grp + 1 - a.window)) {
+        if (pi * KV8_PAGE + KV8_PAGE - 1 > g.pos || (a.window > 0 && pi * KV8_PAGE < g.pos + g.rows - a.window)) {
             kv8_branch();
 #pragma unroll
             for (int q = 0; q < 4; q++)
@@ -625,11 +695,12 @@ DEV void kv8_attend_c16(const cj_kv8_args &a) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) o[j0 + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[j], wl[u], o[j0 + j], 0, 0, 0);
             }
-        if (more) take_v();
     }
 
-    // the four waves' results as one
+    // the four waves' results as one, where the K codes stood
+    float (*so)[KV8_FEW][HD + 4] = (float (*)[KV8_FEW][HD + 4])lds;
     L = kv8_sum4(L);
+    __syncthreads();
 #pragma unroll
     for (int j = 0; j < DT; j++) *(f32x4 *)&so[wv][n][j * 16 + g4 * 4] = o[j];
     if (g4 == 0) {
@@ -637,10 +708,10 @@ DEV void kv8_attend_c16(const cj_kv8_args &a) {
         sl[wv][n] = L;
     }
     __syncthreads();
-    float *part = splits > 1 ? kv8_part<HD>(a, s, h, ct, sp) : nullptr;
+    float *part = splits > 1 ? kv8_part<HD>(a, s, h, 0, sp) : nullptr;
     for (int i = t; i < KV8_FEW * HD / 4; i += 256) {
         const int k = i / (HD / 4), d = i % (HD / 4) * 4;
-        if (c0 + k >= cols) break;
+        if (k >= cols) break;
         const float m = fmaxf(fmaxf(sm[0][k], sm[1][k]), fmaxf(sm[2][k], sm[3][k])), z = m == -INFINITY ? 0.0f : m;
         f32x4 y = {};
         float b = 0;
@@ -657,8 +728,7 @@ DEV void kv8_attend_c16(const cj_kv8_args &a) {
                 part[KV8_FEW * HD + 2 * k + 1] = b;
             }
         } else {
-            const int cc = c0 + k;
-            *(f32x4 *)(a.out + (int64_t)(g.row + cc / grp) * a.out_stride + (int64_t)(h * grp + cc % grp) * HD + d) = y / b;
+            *(f32x4 *)(a.out + (int64_t)(g.row + k / grp) * a.out_stride + (int64_t)(h * grp + k % grp) * HD + d) = y / b;
         }
     }
 }
@@ -733,11 +803,12 @@ struct Kv8Weights {
 #define KV8_SOME 32
 template <int HD>
 DEV void kv8_attend_c32(const cj_kv8_args &a) {
-    constexpr int KS = HD / 16, DT = HD / 32, KW = HD / 32;   // steps, channel tiles, 16-byte words a lane and key
-    constexpr int QB = 2 * KS * 64 * 16, OB = 2 * KV8_SOME * (HD + 4) * 4;
-    __shared__ __align__(16) uint8_t lds[QB > OB ? QB : OB];
-    __shared__ float sm[4][KV8_SOME], sl[4][KV8_SOME];
+    constexpr int KS = HD / 16, DT = HD / 32;   // steps over the channels; channel tiles
+    constexpr int KB = KV8_PAGE * HD, OB = 2 * KV8_SOME * (HD + 4) * 4;
+    __shared__ __align__(16) uint8_t lds[4 * KB > OB ? 4 * KB : OB], qs[2 * KS * 1024];
+    __shared__ float sc[KV8_SOME], sm[4][KV8_SOME], sl[4][KV8_SOME];
     const int t = threadIdx.x, l = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), n = l & 31, hf = l >> 5;
+    // workgroups eight apart share an L2: a segment's column tiles follow one another there
     const uint32_t id = blockIdx.x, per = id / 8 / a.col_tiles, rest = per * 8 + id % 8;
     const int ct = a.col_tiles - 1 - (int)(id / 8 % a.col_tiles);
     const int h = (int)(rest % a.n_kv), sp = (int)(rest / a.n_kv % a.splits), s = (int)(rest / a.n_kv / a.splits);
@@ -750,99 +821,83 @@ DEV void kv8_attend_c32(const cj_kv8_args &a) {
     const int splits = kv8_split(a, g, r0, r1, sp, p0, p1);
     if (sp >= splits) return;
 
-    // this lane's column (past the last: the tile's first again), and its q as halves in LDS
-    const int c = c0 + n < cols ? c0 + n : c0, ri = c / grp;
-    const int last = g.pos + ri, first = a.window > 0 ? last + 1 - a.window : 0;
-    h16x8 *qs = (h16x8 *)lds;
-    float qx[KS][8], top = 0, cs;
+    // q of column t / 8 (past the last: the tile's first again)
+    Kv8Q<HD, KV8_SOME> q;
     {
-        const float *src = a.q + (int64_t)(g.row + ri) * a.q_stride + (int64_t)(h * grp + c % grp) * HD + hf * (HD / 2);
-#pragma unroll
-        for (int k = 0; k < KS; k++) {
-            *(f32x4 *)&qx[k][0] = *(const f32x4 *)(src + 8 * k);
-            *(f32x4 *)&qx[k][4] = *(const f32x4 *)(src + 8 * k + 4);
-        }
+        const int c = c0 + t / 8 < cols ? c0 + t / 8 : c0;
+        q.load(a.q + (int64_t)(g.row + c / grp) * a.q_stride + (int64_t)(h * grp + c % grp) * HD, t % 8);
     }
-    const int key0 = (n >> 2 & 1) * 32 + (n >> 3) * 4 + (n & 3);
-    u32x4 kr[2][KW], vr[2][DT];
+    uint8_t *kl = lds + wv * KB;
+    u32x4 vr[2][DT], vn[2][DT];
     f32x2 ks, vs;
     int pi = p0 + wv;
+    Kv8Table table{a, g.slot, pi, 4, p1, 0};
     bool bad = false;
-    auto page_at = [&](int i) {
-        const int p = kv8_page(a, g.slot, i);
-        bad = p < 0;
-        return (int64_t)(bad ? 0 : p) * a.n_kv + h;
-    };
-    auto load_k = [&](int64_t ph) {
-        const uint8_t *b = a.kc + ph * (KV8_PAGE * HD) + key0 * HD + hf * (HD / 2);
-#pragma unroll
-        for (int q = 0; q < 2; q++)
-#pragma unroll
-            for (int i = 0; i < KW; i++) kr[q][i] = *(const u32x4 *)(b + q * 16 * HD + i * 16);
-        ks = *(const f32x2 *)(a.ks + ph * 4 + 2 * hf);
-    };
-    auto load_v = [&](int64_t ph) {
-        const uint8_t *b = a.vc + ph * (KV8_PAGE * HD) + (2 * hf * HD + n) * 16;
-#pragma unroll
-        for (int q = 0; q < 2; q++)
-#pragma unroll
-            for (int j = 0; j < DT; j++) vr[q][j] = *(const u32x4 *)(b + (q * HD + j * 32) * 16);
-        vs = *(const f32x2 *)(a.vs + ph * 4 + 2 * hf);
-    };
     int64_t ph = 0;
+    auto page_at = [&](int i) {
+        const int p = table.at((i - p0) >> 2);
+        bad = p < 0;
+        ph = (int64_t)(bad ? 0 : p) * a.n_kv + h;
+    };
+    auto copy_k = [&]() {
+        kv8_copy_k<HD>(a.kc + ph * KB, kl, l, [](int row) { return (row >> 2 & 1) * 32 + (row >> 5) * 16 + (row >> 3 & 3) * 4 + (row & 3); });
+    };
+    auto load_v = [&]() {
+        ks = *(const f32x2 *)(a.ks + ph * 4 + 2 * hf);
+        vs = *(const f32x2 *)(a.vs + ph * 4 + 2 * hf);
+        const uint8_t *b = a.vc + ph * KB + (2 * hf * HD + n) * 16;
+#pragma unroll
+        for (int q = 0; q < 2; q++)
+#pragma unroll
+            for (int j = 0; j < DT; j++) vn[q][j] = *(const u32x4 *)(b + (q * HD + j * 32) * 16);
+    };
     if (pi < p1) {
-        ph = page_at(pi);
-        load_k(ph);
-        load_v(ph);
+        page_at(pi);
+        copy_k();
+        load_v();
     }
-    {
-#pragma unroll
-        for (int k = 0; k < KS; k++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(qx[k][i]));
-        int u, v;
-        swap32(__float_as_int(top), u, v);
-        const int e = kv8_q_exponent(fmaxf(__int_as_float(u), __int_as_float(v)));
-        const float sign = a.scale < 0 ? -1.0f : 1.0f;
-        cs = ldexpf(a.scale * sign * KV8_LOG2E, e - 14);
-#pragma unroll
-        for (int k = 0; k < KS; k++) {
-            if (k % 4 != wv) continue;   // (each wave a quarter)
-#pragma unroll
-            for (int i = 0; i < 8; i++) qx[k][i] = ldexpf(qx[k][i] * sign, 14 - e);
-            h16x8 hi, lo;
-            kv8_halves(qx[k], hi, lo);
-            qs[(2 * k) * 64 + l] = hi;
-            qs[(2 * k + 1) * 64 + l] = lo;
-        }
-    }
+    q.store(qs, sc, t / 8, t % 8, a.scale, [t](int d) {
+        return (d % (HD / 2) / 8) * 2048 + (d / (HD / 2) * 32 + t / 8) * 16 + d % 8 * 2;
+    });
+    lds_barrier();
+    const int c = c0 + n < cols ? c0 + n : c0, last = g.pos + c / grp, first = a.window > 0 ? last + 1 - a.window : 0;
+    const float cs = sc[n];
     f32x16 o[DT] = {};
     float M = -INFINITY, L = 0;
-
-    __syncthreads();
     for (; pi < p1; pi += 4) {
+        kv8_landed();
         if (bad && a.status && l == 0) *a.status = 1;
-        f32x16 x[2] = {};
-#pragma unroll
-        for (int k = 0; k < KS; k++) {
-            const h16x8 qh = qs[(2 * k) * 64 + l], ql = qs[(2 * k + 1) * 64 + l];
-            h16x8 f[2];
-#pragma unroll
-            for (int q = 0; q < 2; q++) {
-                const u32x4 w = kr[q][k / 2];
-                f[q] = k & 1 ? kv8_half8(w[2], w[3]) : kv8_half8(w[0], w[1]);
-                x[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[q], qh, x[q], 0, 0, 0);
-            }
-#pragma unroll
-            for (int q = 0; q < 2; q++) x[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[q], ql, x[q], 0, 0, 0);
-        }
         f32x2 kb = ks, vb = vs;
         if (bad) kb[0] = kb[1] = __uint_as_float(0x7fc00000u);
+#pragma unroll
+        for (int q = 0; q < 2; q++)
+#pragma unroll
+            for (int j = 0; j < DT; j++) vr[q][j] = vn[q][j];
         const bool more = pi + 4 < p1;
         if (more) {
-            ph = page_at(pi + 4);
-            load_k(ph);
+            page_at(pi + 4);
+            load_v();
         }
+        f32x16 x[2] = {};
+#pragma unroll
+        for (int k = 0; k < KS; k += 2) {
+            u32x4 w[2];
+#pragma unroll
+            for (int q = 0; q < 2; q++) w[q] = kv8_read_k<HD>(kl, q * 32 + n, hf * (HD / 32) + k / 2);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const h16x8 qh = *(const h16x8 *)(qs + (k + i) * 2048 + l * 16), ql = *(const h16x8 *)(qs + (k + i) * 2048 + 1024 + l * 16);
+                h16x8 f[2];
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    f[q] = kv8_half8(w[q][2 * i], w[q][2 * i + 1]);
+                    x[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[q], qh, x[q], 0, 0, 0);
+                }
+#pragma unroll
+                for (int q = 0; q < 2; q++) x[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[q], ql, x[q], 0, 0, 0);
+            }
+        }
+        if (more) copy_k();
         if (pi * KV8_PAGE + KV8_PAGE - 1 > g.pos + r0 || (a.window > 0 && pi * KV8_PAGE < g.pos + r1 + 1 - a.window))
             kv8_mask(x, kb, vb, pi * KV8_PAGE + hf * 32, first, last);
         Kv8Weights<DT> w(x, kb, vb, cs, M, L, o);
@@ -859,7 +914,6 @@ DEV void kv8_attend_c32(const cj_kv8_args &a) {
                     o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, wl[u], o[j], 0, 0, 0);
                 }
         }
-        if (more) load_v(ph);
     }
 
     // the four waves' results as one: rescaled to the largest maximum, then 2 and 3 onto 0 and 1, then the two
@@ -869,7 +923,7 @@ DEV void kv8_attend_c32(const cj_kv8_args &a) {
         sm[wv][n] = M;
         sl[wv][n] = __int_as_float(u) + __int_as_float(v);
     }
-    __syncthreads();   // (also: q's halves are not read any more)
+    __syncthreads();   // (also: the K codes are not read any more)
     const float z = fmaxf(fmaxf(sm[0][n], sm[1][n]), fmaxf(sm[2][n], sm[3][n])), f = M == -INFINITY ? 0.0f : exp2f(M - z);
     float (*so)[KV8_SOME][HD + 4] = (float (*)[KV8_SOME][HD + 4])lds;
     if (wv >= 2)
@@ -978,8 +1032,9 @@ DEV void kv8_attend_c128(const cj_kv8_args &a) {
     u32x4 kr[CH], vr[CH];
     f32x2 ksn, vsn;
     bool bad = false;
+    Kv8Table table{a, g.slot, p0, 1, p1, 0};
     auto load = [&](int i) {
-        const int p = kv8_page(a, g.slot, i);
+        const int p = table.at(i - p0);
         bad = p < 0;
         const int64_t ph = (int64_t)(bad ? 0 : p) * a.n_kv + h;
         const u32x4 *kb = (const u32x4 *)(a.kc + ph * (KV8_PAGE * HD)), *vb = (const u32x4 *)(a.vc + ph * (KV8_PAGE * HD));
@@ -1080,7 +1135,8 @@ DEV void kv8_join(const cj_kv8_args &a) {
     __shared__ float sm[W], sl[W];
     const int t = threadIdx.x, d = t % C4 * 4, w = t / C4, ways = a.join_ways, per = W / ways, way = w % ways;
     const int grp = a.n_q / a.n_kv, most = a.max_rows * grp, tiles = (most + per - 1) / per;
-    const int h = blockIdx.x / tiles % a.n_kv, s = blockIdx.x / tiles / a.n_kv, c = blockIdx.x % tiles * per + w / ways;
+    const uint32_t id = blockIdx.x;
+    const int h = (int)(id % a.n_kv), s = (int)(id / a.n_kv / tiles), c = (int)(id / a.n_kv % tiles) * per + w / ways;
     Kv8Seg g;
     if (!kv8_seg(a, s, g)) return;
     const int cols = g.rows * grp, tc = a.tile_cols, ct = c / tc, k = c - ct * tc, c0 = ct * tc;

@@ -174,7 +174,7 @@ int32_t cj_kv8_attend(int64_t out, int64_t q, int64_t kplane, int64_t vplane, in
     int64_t ways = 1, W = 1024 / head_dim;
     while (ways < W && ways < p.splits) ways *= 2;
     const int64_t units = (int64_t)n_segs * n_kv * p.splits, per = W / ways, cols = (int64_t)max_rows * (n_q / n_kv);
-    const int64_t wgs = (p.tile_cols == 128 ? units : (units + 7) / 8 * 8) * p.col_tiles, join = (int64_t)n_segs * n_kv * ((cols + per - 1) / per);
+    const int64_t wgs = (p.tile_cols == 32 ? (units + 7) / 8 * 8 : units) * p.col_tiles, join = (int64_t)n_segs * n_kv * ((cols + per - 1) / per);
     if (wgs > 0x7fffffff || join > 0x7fffffff)
         return fail(CJ_ERR_ARG, "cj_kv8_attend: %d x %d rows of %d heads exceed a launch", n_segs, max_rows, n_q);
     a.part = (float *)dptr(part); a.col_tiles = (int32_t)p.col_tiles; a.tile_cols = (int32_t)p.tile_cols;
