@@ -25,11 +25,13 @@ struct Kv8Seg {
     int slot, pos, row, rows;
 };
 
-// The segment s, and whether its slot, rows and positions are in range.
+// The segment s; false where it has no rows, or where its slot, rows or
+// positions are out of range, which is reported.
 DEV bool kv8_seg(const cj_kv8_args &a, int s, Kv8Seg &g) {
     const int4 v = ((const int4 *)a.segs)[s];
     g.slot = v.x; g.pos = v.y; g.row = v.z; g.rows = v.w;
-    const bool ok = v.x >= 0 && v.x < a.n_slots && v.w >= 0 && v.w <= a.max_rows && v.z >= 0 && v.z <= a.n_rows - v.w &&
+    if (v.w == 0) return false;
+    const bool ok = v.x >= 0 && v.x < a.n_slots && v.w > 0 && v.w <= a.max_rows && v.z >= 0 && v.z <= a.n_rows - v.w &&
                     v.y >= 0 && v.y <= a.limit - v.w;
     if (!ok && a.status && threadIdx.x == 0) *a.status = 1;
     return ok;
@@ -191,8 +193,8 @@ DEV void kv8_append(const cj_kv8_args &a) {
     const int nb = (a.max_rows + KV8_BLOCK - 2) / KV8_BLOCK + 1;
     const int h = blockIdx.x % a.n_kv, w = blockIdx.x / a.n_kv, blk = w % nb, s = w / nb;
     if (!kv8_seg(a, s, g)) return;
+    if (blk > (g.pos + g.rows - 1) / KV8_BLOCK - g.pos / KV8_BLOCK) return;
     const int b0 = (g.pos / KV8_BLOCK + blk) * KV8_BLOCK;
-    if (g.rows == 0 || b0 >= g.pos + g.rows) return;
     // a slot has one segment in a call: two would write one block at once
     int twice = 0;
     for (int i = t; i < a.n_segs; i += 256) {
@@ -310,8 +312,8 @@ DEV void kv8_read(const cj_kv8_args &a) {
     const int h = blockIdx.x % a.n_kv, w = blockIdx.x / a.n_kv, blk = w % nb, s = w / nb;
     Kv8Seg g;
     if (!kv8_seg(a, s, g)) return;
+    if (blk > (g.pos + g.rows - 1) / KV8_BLOCK - g.pos / KV8_BLOCK) return;
     const int b0 = (g.pos / KV8_BLOCK + blk) * KV8_BLOCK;
-    if (b0 >= g.pos + g.rows) return;
     int page = kv8_page(a, g.slot, b0 / KV8_PAGE);
     const bool bad = page < 0;
     if (bad) {
@@ -553,7 +555,6 @@ DEV void kv8_attend_c16(const cj_kv8_args &a) {
     Kv8Seg g;
     if (!kv8_seg(a, s, g)) return;
     const int grp = a.n_q / a.n_kv, cols = g.rows * grp;
-    if (cols == 0) return;
     int p0, p1;
     const int splits = kv8_split(a, g, 0, g.rows - 1, sp, p0, p1);
     if (sp >= splits) return;

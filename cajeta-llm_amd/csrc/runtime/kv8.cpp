@@ -29,6 +29,8 @@ int common(const char *who, cj_kv8_args &a, int64_t kplane, int64_t vplane, int6
     if (!shape_ok(n_q, n_kv, hd)) return fail(CJ_ERR_ARG, "%s: heads %d/%d of size %d are not served", who, n_q, n_kv, hd);
     if (n_segs <= 0 || max_rows <= 0 || n_rows <= 0)
         return fail(CJ_ERR_ARG, "%s: %d segments of up to %d rows, %d rows", who, n_segs, max_rows, n_rows);
+    if ((int64_t)max_rows * n_q > (1 << 30))
+        return fail(CJ_ERR_ARG, "%s: %d rows of %d heads exceed a launch", who, max_rows, n_q);
     if (n_pages <= 0 || n_slots <= 0 || slot_pages <= 0 || slot_pages > 0x7fffffff / 64)
         return fail(CJ_ERR_ARG, "%s: %d pages, %d slots of %d pages", who, n_pages, n_slots, slot_pages);
     if (!ready()) return fail(CJ_ERR_STATE, "cj_init has not run");
@@ -52,8 +54,9 @@ int common(const char *who, cj_kv8_args &a, int64_t kplane, int64_t vplane, int6
 // Blocks of 16 positions that max_rows rows reach at most.
 int64_t blocks_of(int32_t max_rows) { return ((int64_t)max_rows + 14) / 16 + 1; }
 
+// (A launch holds fewer than 2^32 threads.)
 int run(const char *kernel, int32_t hd, int64_t grid, uint32_t block, const cj_kv8_args &a) {
-    if (grid > 0x7fffffff) return fail(CJ_ERR_ARG, "%s: %lld workgroups exceed a launch", kernel, (long long)grid);
+    if (grid > 0xffffffffll / block) return fail(CJ_ERR_ARG, "%s: %lld workgroups exceed a launch", kernel, (long long)grid);
     return launch((std::string(kernel) + "_h" + std::to_string(hd)).c_str(), (uint32_t)grid, block, 0, a);
 }
 
@@ -146,7 +149,7 @@ int32_t cj_kv8_read(int64_t k_out, int64_t v_out, int64_t kplane, int64_t vplane
 
 int64_t cj_kv8_attend_bytes(int32_t n_segs, int32_t max_rows, int32_t max_count, int32_t n_q, int32_t n_kv, int32_t head_dim,
                             int32_t window) {
-    if (!shape_ok(n_q, n_kv, head_dim) || n_segs <= 0 || max_rows <= 0 || max_count <= 0 || window < 0)
+    if (!shape_ok(n_q, n_kv, head_dim) || n_segs <= 0 || max_rows <= 0 || (int64_t)max_rows * n_q > (1 << 30) || max_count <= 0 || window < 0)
         return fail(CJ_ERR_ARG, "cj_kv8_attend_bytes: %d segments of %d rows, %d positions, heads %d/%d of size %d", n_segs,
                     max_rows, max_count, n_q, n_kv, head_dim);
     if (!ready()) return fail(CJ_ERR_STATE, "cj_init has not run");   // the split follows the device's size

@@ -282,8 +282,8 @@ int32_t cj_attn_scores(int64_t scores, int64_t q, int64_t kcache, int64_t pgtab,
  * The calls work on n_segs segments: device int32 {slot, pos, row, rows}
  * each: rows row .. row + rows of the row buffers are the positions pos ..
  * pos + rows of the sequence in `slot`, whose pages stand in pgtab[slot]
- * [0 .. slot_pages), one of [n_slots][slot_pages] rows. A segment may hold
- * no rows; rows of no segment are left as they are. The segments and the
+ * [0 .. slot_pages), one of [n_slots][slot_pages] rows. A segment of no rows
+ * is passed over; rows of no segment are left as they are. The segments and the
  * page table are read on the device in stream order, so a captured graph
  * follows their contents. A segment outside its bounds (slot < n_slots, rows
  * <= max_rows, row + rows <= n_rows, positions within the slot's pages) is
@@ -322,7 +322,7 @@ int32_t cj_kv8_read(int64_t k_out, int64_t v_out, int64_t kplane, int64_t vplane
  * h / (n_q / n_kv). No segment ends past max_count. `part` holds the partial
  * results where the positions are split over workgroups:
  * cj_kv8_attend_bytes bytes (with the same arguments; 0: none, and part may
- * be 0). Accurate to f32: the rows and weights enter the f16 matrix cores as
+ * be 0); calls of two threads at once need one each. Accurate to f32: the rows and weights enter the f16 matrix cores as
  * two halves each, codes are exact in f16. Segments of one row and long
  * chunks may share a call; each is fastest in a call of its own kind.
  * Beside cj_attend (one row of one sequence, fp16 planes). */

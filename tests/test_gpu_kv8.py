@@ -283,8 +283,10 @@ def test_refused_segments_are_skipped_and_reported(gpu):
     assert P.stat() == 1
     P.ref.append(3, 30, turned(k[2:4].astype(np.float64), P.rope, 30), v[2:4].astype(np.float64))
     P.check_read()
-    # without rows it may stand there twice
-    P.append([(1, 30, 0, 2), (1, 30, 2, 0)], q, k, v, model=False)
+    # without rows it may stand there twice, and a segment without rows may say anything
+    P.append([(1, 30, 0, 2), (1, 30, 2, 0), (-1, -2 ** 31, 2 ** 31 - 1, 0)], q, k, v, model=False)
+    assert (P.read([(7, 2 ** 31 - 1, -5, 0)], n=3)[0] == MARK).all()
+    assert (P.attend([(-1, 2 ** 31 - 16, -5, 0), (9, 0, 0, 0)], q, max_count=100)[0] == MARK).all()
     assert P.stat() == 0
     P.ref.append(1, 30, turned(k[:2].astype(np.float64), P.rope, 30), v[:2].astype(np.float64))
     P.check_read()
@@ -455,6 +457,29 @@ def test_a_pool_past_four_gigabytes(gpu):
     assert P.stat() == 0
 
 
+def test_positions_near_two_to_the_31(gpu):
+    """A slot of 2^25 pages, of which the last few exist, and a bound on the rows that would wrap a position."""
+    rng = np.random.default_rng(6)
+    heads, kv, hd, L = 4, 1, 64, gpu.native.lib()
+    P = Pages(gpu, heads, kv, hd, 1, 4, pool=9)
+    P.append([(0, 0, 0, 200)], *rows_of(rng, 200, heads, kv, hd))
+    want = P.read([(0, 0, 0, 200)])
+    pages = (2 ** 31 - 1) // 64
+    table = np.full((1, pages), -1, np.int32)
+    table[0, -4:] = P.table[0]
+    base = (pages - 4) * 64
+    P.tab, P.slot_pages = gpu.Buffer.of(table), pages
+    got = P.read([(0, base, 0, 200)], max_rows=2 ** 27)
+    assert all(np.array_equal(x, y) for x, y in zip(got, want))
+    for rows in (1, 7, 40):      # the rows that a window lets see the four pages alone
+        q = rows_of(rng, rows, heads, kv, hd)[0]
+        got, scale = P.attend([(0, base + 200 - rows, 0, rows)], q, window=100)
+        ref, tol = attention(q.astype(np.float64), P.ref.values(0, "k", 0, 200), P.ref.values(0, "v", 0, 200), 200 - rows, scale,
+                             100, P.ref.steps(0, "v").repeat(BLOCK, 0))
+        assert (np.abs(got - ref) <= tol).all()
+    assert P.stat() == 0
+
+
 def serve(P, rng, steps, lens, attend=True):
     """Prompts in chunks of uneven sizes, then decode steps, as a serving loop runs them."""
     heads, kv, hd = P.heads, P.kv, P.hd
@@ -577,15 +602,13 @@ def test_refusals(gpu):
                    dict(rope_ctx=0), dict(rope_ctx=P.ctx + 1), dict(qw=0), dict(kw=0), dict(q_stride=heads * hd - 4),
                    dict(q_stride=heads * hd + 1), dict(kv_stride=kv * hd - 4), dict(kv_stride=-kv * hd),
                    dict(q_out_stride=2 ** 62), dict(n_q=7), dict(n_q=0), dict(n_q=65 * kv)],
-        "read": [dict(k_out=0, v_out=0), dict(k_out=k.h + 4), dict(out_stride=kv * hd + 4), dict(out_stride=2)],
+        "read": [dict(k_out=0, v_out=0), dict(max_rows=2 ** 28), dict(k_out=k.h + 4), dict(out_stride=kv * hd + 4), dict(out_stride=2)],
         "attend": [dict(out=0), dict(q=0), dict(q=q.h + 8), dict(max_count=0), dict(window=-1), dict(n_q=7), dict(n_q=65 * kv),
-                   dict(out_stride=heads * hd + 4), dict(q_stride=heads * hd - 64), dict(max_rows=2 ** 31 - 1, n_segs=2)],
+                   dict(out_stride=heads * hd + 4), dict(q_stride=heads * hd - 64), dict(max_rows=2 ** 31 - 1)],
     }
     for name in ("append", "read", "attend"):
         assert call(name) == 0, (name, gpu.native.last_error())
         for change in both + extra[name]:
-            if name == "attend" and "n_segs" in change and "max_rows" in change:
-                continue
             assert call(name, **change) == ARG, (name, change)
             assert ("cj_kv8_" + name) in gpu.native.last_error(), (name, change)
     # the queries, the norm and one of the outputs may be left out
