@@ -459,11 +459,11 @@ DEV float *kv8_part(const cj_kv8_args &a, int s, int h, int ct, int sp) {
 // loaded, each would cost the wave a round trip to memory.
 struct Kv8Table {
     const cj_kv8_args &a;
-    const int slot, from, step, end;   // pages from, from + step, .. before end
+    const int slot, from, end;   // pages from, from + 4, .. before end
     int ids;
-    // the id of page from + step·k (k from 0 up, one after the other), −1 where there is none
+    // the id of page from + 4k (k from 0 up, one after the other), −1 where there is none
     DEV int at(int k) {
-        if ((k & 63) == 0) ids = kv8_page(a, slot, min(end - 1, from + step * (k + (int)(threadIdx.x & 63))));
+        if ((k & 63) == 0) ids = kv8_page(a, slot, min(end - 1, from + 4 * (k + (int)(threadIdx.x & 63))));
         return __builtin_amdgcn_readlane(ids, k & 63);
     }
 };
@@ -569,7 +569,7 @@ DEV void kv8_attend_c16(const cj_kv8_args &a) {
     u32x4 vr[DT], vn[DT];
     float ks, vs;
     int pi = p0 + wv;
-    Kv8Table table{a, g.slot, pi, 4, p1, 0};
+    Kv8Table table{a, g.slot, pi, p1, 0};
     bool bad = false;
     int64_t ph = 0;
     auto page_at = [&](int i) {
@@ -647,10 +647,8 @@ DEV void kv8_attend_c16(const cj_kv8_args &a) {
 #pragma unroll
             for (int q = 0; q < 4; q++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int p = at + 4 * q + i;
-                    x[q][i] = p <= last && p >= first ? __builtin_fmaf(x[q][i], kf, ve) : -INFINITY;
-                }
+                for (int i = 0; i < 4; i++)
+                    x[q][i] = (uint32_t)(at - first + 4 * q + i) <= (uint32_t)(last - first) ? __builtin_fmaf(x[q][i], kf, ve) : -INFINITY;
         } else {
 #pragma unroll
             for (int q = 0; q < 4; q++)
@@ -739,11 +737,13 @@ DEV void kv8_attend_c16(const cj_kv8_args &a) {
 // it sees nothing may have no scale.
 DEV void kv8_mask(f32x16 (&x)[2], f32x2 &ks, f32x2 &vs, int p, int first, int last) {
     kv8_branch();
+    const uint32_t seen = (uint32_t)(last - first);
 #pragma unroll
     for (int q = 0; q < 2; q++, p += 16) {
+        const uint32_t at = (uint32_t)(p - first);   // (before first: past any `seen`)
 #pragma unroll
         for (int i = 0; i < 16; i++)
-            if (p + i > last || p + i < first) x[q][i] = -INFINITY;
+            if (at + i > seen) x[q][i] = -INFINITY;
         if (p > last || p + 15 < first) ks[q] = vs[q] = 1.0f;
     }
 }
@@ -832,7 +832,7 @@ DEV void kv8_attend_c32(const cj_kv8_args &a) {
     u32x4 vr[2][DT], vn[2][DT];
     f32x2 ks, vs;
     int pi = p0 + wv;
-    Kv8Table table{a, g.slot, pi, 4, p1, 0};
+    Kv8Table table{a, g.slot, pi, p1, 0};
     bool bad = false;
     int64_t ph = 0;
     auto page_at = [&](int i) {
@@ -1033,9 +1033,8 @@ DEV void kv8_attend_c128(const cj_kv8_args &a) {
     u32x4 kr[CH], vr[CH];
     f32x2 ksn, vsn;
     bool bad = false;
-    Kv8Table table{a, g.slot, p0, 1, p1, 0};
     auto load = [&](int i) {
-        const int p = table.at(i - p0);
+        const int p = kv8_page(a, g.slot, i);
         bad = p < 0;
         const int64_t ph = (int64_t)(bad ? 0 : p) * a.n_kv + h;
         const u32x4 *kb = (const u32x4 *)(a.kc + ph * (KV8_PAGE * HD)), *vb = (const u32x4 *)(a.vc + ph * (KV8_PAGE * HD));
