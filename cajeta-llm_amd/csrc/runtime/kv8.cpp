@@ -63,16 +63,19 @@ int run(const char *kernel, int32_t hd, int64_t grid, uint32_t block, const cj_k
 // How a call runs. A column is a row and a query head of one kv head's group;
 // a workgroup takes 16, 32 or 128 of a segment's and, up to 32, a part of the
 // positions (a wave a page at a time), whose parts a second launch joins.
-// Measured on 256 CUs at head size 128, 4 heads a kv head, 8 kv heads:
-//  - 128 columns a workgroup convert a page once for four waves, but keep a
-//    chip of 256 CUs busy only where there are enough of them (us, 32 → 128;
-//    1024 rows behind 1033, 256 workgroups of 128: 77 → 80; 1536 rows, 384:
-//    121 → 114; 2048 rows, 512: 171 → 150);
-//  - the positions are split for two workgroups a CU, what fits one (one
-//    sequence of 65500: 32.7 us, for one 35.4, three 36.6, six 41.6; 32
-//    sequences of 16384: 177, 196, 182, 183), and not where it saves a wave
-//    two pages or less, about 2 us each, for the join's 4 us (32 sequences of
-//    1024, a split or none: 23.6 and 17.6; one of 257: 10.9 and 8.3).
+// Measured on 256 CUs at head size 128, 4 heads a kv head, 8 kv heads (us):
+//  - 128 columns a workgroup convert a page once for four waves, but keep the
+//    chip busy only where there are enough of them (32 → 128; 1024 rows behind
+//    1033, 256 workgroups of 128: 73 → 81 stays; 1536 rows, 384: 117 → 112;
+//    2048 rows, 512: 162 → 150);
+//  - the positions are split for one workgroup a CU (for one and for two; 32
+//    sequences of 2048: 25 and 29; of 4096: 46 and 52; 8 of 65500: 170 and
+//    172; one: 30 and 31; 24 of 8192: 69 and 76), and not where it saves a
+//    wave two pages or less for the join's 3 us (one sequence of 513, no split
+//    and one: 8.8 and 9.6; of 1025, 12.2 and 10.5);
+//  - a little over one workgroup a CU would leave a few CUs two of them: long
+//    ones are split in three (none and three; 33 sequences of 6000: 93 and 81,
+//    40: 97 and 88, but 50: 106 and 115; 33 of 2048: 34 and 35).
 struct Plan {
     int64_t tile_cols, col_tiles, splits, split_pages, bytes;
 };
@@ -83,7 +86,9 @@ Plan plan_attend(int64_t n_segs, int64_t max_rows, int64_t max_count, int64_t n_
     p.col_tiles = (cols + p.tile_cols - 1) / p.tile_cols;
     int64_t pages = (max_count + 63) / 64;
     if (window) pages = std::min(pages, (window + max_rows) / 64 + 2);   // what a tile's rows see together
-    const int64_t units = heads * p.col_tiles, want = std::max<int64_t>(1, 2 * cus / units);
+    const int64_t units = heads * p.col_tiles;
+    int64_t want = std::max<int64_t>(1, cus / units);
+    if (p.tile_cols == 16 && units > cus && 3 * units <= 4 * cus && pages >= 64) want = 3;
     p.split_pages = std::max<int64_t>(4, (pages + want - 1) / want);
     if (p.tile_cols == 128 || pages <= p.split_pages + 8) p.split_pages = pages;
     p.splits = (pages + p.split_pages - 1) / p.split_pages;
