@@ -154,7 +154,11 @@ DEV uint32_t kv8_code(double x, double inv) { return (uint32_t)((int)rint(x * in
 
 // Append: a workgroup a (segment, block, kv head), thread t position t / 16
 // of the block and its rotation pairs (t % 16)·NP.., so a head's row is 16
-// lanes; then workgroups of (row, query head) pairs, 16 bytes a lane.
+// lanes; then workgroups of (row, query head) pairs, 16 bytes a lane (8 bytes
+// a lane at head size 64: 37 → 33 us).
+// Bound: HBM for many rows (3130 rows of 64 / 8 heads of 64 with the norm: 32
+// us, 3.7 TB/s; without 29; q's rows alone 22), a launch for few. The 64-bit
+// arithmetic costs the norm's 3 us and nothing else.
 template <int HD>
 DEV void kv8_append(const cj_kv8_args &a) {
     constexpr int NP = HD / 32;
@@ -214,7 +218,7 @@ DEV void kv8_append(const cj_kv8_args &a) {
     double kx[NP], ky[NP], vx[NP], vy[NP];
     double ktop = 0, vtop = 0;
     if (fresh) {
-        const int64_t at = (int64_t)(g.row + p - g.pos) * a.kv_stride + (int64_t)h * HD + j * NP;
+        const int64_t at = (int64_t)(g.row + (p - g.pos)) * a.kv_stride + (int64_t)h * HD + j * NP;
         kv8_load<NP>(a.k + at, kx);
         kv8_load<NP>(a.k + at + HD / 2, ky);
         kv8_load<NP>(a.v + at, vx);
@@ -302,7 +306,8 @@ DEV void kv8_append(const cj_kv8_args &a) {
 }
 
 // Read: a workgroup a (segment, block, kv head); thread t the position t / 16
-// and HD / 16 of its channels.
+// and HD / 16 of its channels, V through LDS. Bound: HBM (3300 positions of 8
+// heads of 64 in 6.5 us, 2.6 TB/s), a launch for few.
 template <int HD>
 DEV void kv8_read(const cj_kv8_args &a) {
     constexpr int W = HD / 16;
@@ -327,7 +332,7 @@ DEV void kv8_read(const cj_kv8_args &a) {
     const int p = b0 + tt;
     if (p < g.pos || p >= g.pos + g.rows) return;
     const float none = __uint_as_float(0x7fc00000u), ks = bad ? none : a.ks[si], vs = bad ? none : a.vs[si];
-    const int64_t o = (int64_t)(g.row + p - g.pos) * a.out_stride + (int64_t)h * HD + j * W;
+    const int64_t o = (int64_t)(g.row + (p - g.pos)) * a.out_stride + (int64_t)h * HD + j * W;
     if (a.out)
 #pragma unroll
         for (int i = 0; i < W; i += 4) {
@@ -456,7 +461,8 @@ DEV float *kv8_part(const cj_kv8_args &a, int s, int h, int ct, int sp) {
 }
 
 // Page ids of a run of pages, 64 at a time, one a lane: read where a page is
-// loaded, each would cost the wave a round trip to memory.
+// loaded, each would cost the wave a round trip to memory (8 sequences of
+// 65500: 177 us, so 170).
 struct Kv8Table {
     const cj_kv8_args &a;
     const int slot, from, end;   // pages from, from + 4, .. before end
@@ -469,8 +475,9 @@ struct Kv8Table {
 };
 
 // A page's K codes go from memory straight into the wave's part of LDS, eight
-// (HD 128) or four lanes a row, so that a copy touches whole lines (a lane a
-// row, 64 lines an instruction, cost the c32 kernel more than its products).
+// (HD 128) or four lanes a row, so that a copy touches whole lines. (A lane a
+// row, 64 lines an instruction: 32 ragged sequences of up to 4096 positions
+// 44.8 us, so 35.6; 64 rows behind 1033 24 and 19.6.)
 // LDS row ρ holds key `key(ρ)` of the page; its 16-byte word c stands at c ^
 // swizzle(ρ), so that eight rows' reads of one word fall on all banks once.
 template <int HD>
@@ -534,15 +541,19 @@ struct Kv8Q {
     }
 };
 
-// Few columns (a column is a row and one query head of the kv head's group):
-// a workgroup a (segment, kv head, 16 columns, split), its four waves a page
-// each in turn. All operands come straight from memory to registers, in the
-// order that makes the scores' accumulators the next product's operand:
+// Few columns (a column is a row and one query head of the kv head's group;
+// up to 16): a workgroup a (segment, kv head, split), its four waves a page
+// each in turn. The tiles' rows are placed so that the scores' accumulators
+// are the next product's operand as they lie:
 //  - scores: A rows are keys, row m of tile t is position (m/4)·16 + 4t + m%4
 //    of the page, so lane group g = l/16 gets its 16 positions of block g in
 //    order, and one K and one V scale a lane;
-//  - output: B is the weights as they lie, A the V codes, 16 positions of a
-//    channel in 16 bytes.
+//  - output: B is the weights, A the V codes, 16 positions of a channel in 16
+//    bytes, a page ahead in registers.
+// Bound: HBM where there is enough to read (8 sequences of 65500 positions, 8
+// kv heads of 128: 171 us, 6.27 TB/s; 32 ragged ones of up to 4096: 33 us,
+// 4.8 TB/s with the join, ramp and tail), else the chain of round trips
+// (segment, page table, page, output: 6.6 us for one of 2049, and the join).
 template <int HD>
 DEV void kv8_attend_c16(const cj_kv8_args &a) {
     constexpr int KS = HD / 32, DT = HD / 16;   // steps over the channels; channel tiles
@@ -797,10 +808,14 @@ struct Kv8Weights {
 };
 
 // Some columns (17 and more, where 128 a workgroup would leave the chip
-// empty): as for few, every wave its own pages straight from memory, but 32
-// columns and the 32-row products. q's halves stand in LDS, being the same
-// for all waves. Tile q's row r is position 32·(r/4 % 2) + 16q + 4·(r/8) +
-// r%4, which gives lane half h = l/32 blocks 2h and 2h + 1 in order.
+// empty): as for few, every wave its own pages, but 32 columns and the 32-row
+// products. q's halves stay in LDS, being the same for all waves. Tile q's row
+// r is position 32·(r/4 % 2) + 16q + 4·(r/8) + r%4, which gives lane half h =
+// l/32 blocks 2h and 2h + 1 in order.
+// Bound: the waves' own work, VALU (the codes' conversion, once a wave, and
+// the softmax: 39% of the cycles) and matrix cores (27%) hardly overlapping
+// (512 rows behind 1545 of 32 / 8 heads of 128: 38 us, 400 TFLOP/s; three rows
+// of 16 sequences of 4097, 64 / 8 heads of 64: 18 us and the join's 5).
 #define KV8_SOME 32
 template <int HD>
 DEV void kv8_attend_c32(const cj_kv8_args &a) {
@@ -975,12 +990,15 @@ DEV void kv8_attend_c32(const cj_kv8_args &a) {
 // columns), a wave 32 columns, every wave over the same pages. A page's codes
 // become f16 once, on their way into LDS, and serve the four waves; the next
 // page's codes are on their way to registers meanwhile, so a page costs one
-// barrier. As above, the tiles' rows are placed so that lane half h = l/32
-// gets blocks 2h and 2h + 1 of the page in order and the scores' accumulators
-// are the weights' operand as they lie.
+// barrier. Rows as above.
 //  - K in LDS: row 32t + r of 16-byte words, word c at c ^ (row & 15), so that
-//    eight lanes' rows lie in different banks;
+//    16 lanes' rows lie in different banks;
 //  - V in LDS: [t][u][h][channel] words of the 8 positions 8u.. of block 2h + t.
+// Bound: the matrix cores' power: four prompts of 4096 rows, 32 / 8 heads of
+// 128, in 985 us are 1.12 PFLOP/s of f16 products (two for each one of the
+// attention's, whose 560 TFLOP/s that makes) at 1.8 GHz, where an 8192^3 f16
+// product of the library reaches 1.15. In a 128-position window (16 prompts of
+// up to 300 rows, 64 / 8 heads of 64: 36 us) the softmax's VALU work.
 #define KV8_MANY 128
 template <int HD>
 DEV void kv8_attend_c128(const cj_kv8_args &a) {
@@ -1127,7 +1145,9 @@ DEV void kv8_attend_c128(const cj_kv8_args &a) {
 
 // The splits of the columns as one row each: HD / 4 threads a channel group,
 // a.join_ways of them side by side over a column's splits, which are then
-// joined in order; the other threads of the workgroup are other columns.
+// joined in order; the other threads of the workgroup are other columns. kv
+// head = id mod n_kv, as the parts were written, so that they are read through
+// the L2 that holds them. Bound: a launch (3 to 5 us).
 template <int HD>
 DEV void kv8_join(const cj_kv8_args &a) {
     constexpr int C4 = HD / 4, W = 256 / C4;

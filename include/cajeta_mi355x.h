@@ -319,7 +319,7 @@ int32_t cj_kv8_read(int64_t k_out, int64_t v_out, int64_t kplane, int64_t vplane
 /* Causal attention of the segments' q rows over their cached positions: the
  * row at position p attends [max(0, p + 1 - window), p] (window 0: all), its
  * own position, appended before, included; query head h reads kv head
- * h / (n_q / n_kv). No segment ends past max_count. `part` holds the partial
+ * h / (n_q / n_kv). `out` may be `q` (with the same strides). No segment ends past max_count. `part` holds the partial
  * results where the positions are split over workgroups:
  * cj_kv8_attend_bytes bytes (with the same arguments; 0: none, and part may
  * be 0); calls of two threads at once need one each. Accurate to f32: the rows and weights enter the f16 matrix cores as

@@ -563,6 +563,30 @@ def test_a_captured_step_follows_its_segments_and_tables(gpu):
     assert P.stat() == 0
 
 
+@pytest.mark.parametrize("rows,count", [(1, 100), (1, 2049), (12, 2049), (200, 300)])
+def test_out_may_be_q(gpu, rows, count):
+    rng = np.random.default_rng(rows)
+    heads, kv, hd, L = 32, 8, 128, gpu.native.lib()
+    P = Pages(gpu, heads, kv, hd, 1, 33)
+    P.append([(0, 0, 0, count)], *rows_of(rng, count, heads, kv, hd))
+    q = rows_of(rng, rows, heads, kv, hd)[0]
+    want, scale = P.attend([(0, count - rows, 0, rows)], q)
+    b, sb = gpu.Buffer.of(q), P.segs([(0, count - rows, 0, rows)])
+    need = L.cj_kv8_attend_bytes(1, rows, count, heads, kv, hd, 0)
+    part = gpu.Buffer(max(16, need))
+    gpu.native.check(L.cj_kv8_attend(
+        b.h, b.h, P.planes[0].h, P.planes[1].h, P.tab.h, sb.h, part.h, 1, rows, rows, count, P.pool, P.slots, P.slot_pages, heads,
+        kv, hd, heads * hd, heads * hd, 0, ctypes.c_float(scale), P.status.h), "attend")
+    assert np.array_equal(b.download(np.float32, q.size).reshape(q.shape), want)
+    # a workspace that is too small is refused before anything runs
+    if need:
+        small = gpu.Buffer(need - 16)
+        assert L.cj_kv8_attend(
+            b.h, b.h, P.planes[0].h, P.planes[1].h, P.tab.h, sb.h, small.h, 1, rows, rows, count, P.pool, P.slots, P.slot_pages,
+            heads, kv, hd, heads * hd, heads * hd, 0, ctypes.c_float(scale), P.status.h) == gpu.native.CJ_ERR_ARG
+        assert "part" in gpu.native.last_error()
+
+
 def test_refusals(gpu):
     """Arguments that the host refuses before anything is launched."""
     L, ARG = gpu.native.lib(), gpu.native.CJ_ERR_ARG
