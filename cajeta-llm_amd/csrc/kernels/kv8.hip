@@ -479,9 +479,9 @@ struct Kv8Table {
 // row, 64 lines an instruction: 32 ragged sequences of up to 4096 positions
 // 44.8 us, so 35.6; 64 rows behind 1033 24 and 19.6.)
 // LDS row ρ holds key `key(ρ)` of the page; its 16-byte word c stands at c ^
-// swizzle(ρ), so that eight rows' reads of one word fall on all banks once.
+// swizzle(ρ), so that 16 rows' reads of one word fall on all 64 banks once.
 template <int HD>
-DEV int kv8_swizzle(int row) { return HD == 128 ? row & 7 : row >> 2 & 3; }
+DEV int kv8_swizzle(int row) { return HD == 128 ? row >> 1 & 7 : row >> 2 & 3; }
 template <int HD, class Key>
 DEV void kv8_copy_k(const uint8_t *page, uint8_t *lds, int l, Key &&key) {
     constexpr int W = HD / 16;   // words a row
@@ -552,8 +552,8 @@ struct Kv8Q {
 //    bytes, a page ahead in registers.
 // Bound: HBM where there is enough to read (8 sequences of 65500 positions, 8
 // kv heads of 128: 171 us, 6.27 TB/s; 32 ragged ones of up to 4096: 33 us,
-// 4.8 TB/s with the join, ramp and tail), else the chain of round trips
-// (segment, page table, page, output: 6.6 us for one of 2049, and the join).
+// 5.05 TB/s with ramp and tail), else the chain of round trips (segment, page
+// table, page, output: 6 us for one of 2049, and the join's 3).
 template <int HD>
 DEV void kv8_attend_c16(const cj_kv8_args &a) {
     constexpr int KS = HD / 32, DT = HD / 16;   // steps over the channels; channel tiles
@@ -813,8 +813,8 @@ struct Kv8Weights {
 // r is position 32·(r/4 % 2) + 16q + 4·(r/8) + r%4, which gives lane half h =
 // l/32 blocks 2h and 2h + 1 in order.
 // Bound: the waves' own work, VALU (the codes' conversion, once a wave, and
-// the softmax: 39% of the cycles) and matrix cores (27%) hardly overlapping
-// (512 rows behind 1545 of 32 / 8 heads of 128: 38 us, 400 TFLOP/s; three rows
+// the softmax: 45% of the cycles) and matrix cores (28%) hardly overlapping
+// (512 rows behind 1545 of 32 / 8 heads of 128: 41 us, 370 TFLOP/s; three rows
 // of 16 sequences of 4097, 64 / 8 heads of 64: 18 us and the join's 5).
 #define KV8_SOME 32
 template <int HD>
