@@ -563,6 +563,48 @@ def test_a_captured_step_follows_its_segments_and_tables(gpu):
     assert P.stat() == 0
 
 
+def test_beside_the_fp16_planes(gpu):
+    """The same token through cj_qk_prep and cj_attend over fp16 planes: q by the same table, and an attention that differs
+    by what eight bits lose of K and V."""
+    L, check, f = gpu.native.lib(), gpu.native.check, ctypes.c_float
+    rng = np.random.default_rng(12)
+    heads, kv, hd, count = 32, 8, 128, 150
+    P = Pages(gpu, heads, kv, hd, 1, 3, pool=3)
+    check(L.cj_rope_table(P.rope_b.h, hd, f(10000.0), P.ctx), "rope table")
+    P.rope = P.rope_b.download(np.float32, P.ctx * hd).reshape(P.ctx, hd // 2, 2)
+    q, k, v = rows_of(rng, count, heads, kv, hd)
+    got, want = P.append([(0, 0, 0, count)], q, k, v)
+    assert near(got, want)
+    kc, vc = gpu.Buffer(3 * kv * 64 * hd * 2), gpu.Buffer(3 * kv * 64 * hd * 2)
+    part, cnt, out = gpu.Buffer(heads * 64 * (hd + 2) * 4), gpu.Buffer(kv * 4), gpu.Buffer(heads * hd * 4)
+    cnt.zero()
+    for t in range(count):
+        qb, kb, vb = gpu.Buffer.of(q[t]), gpu.Buffer.of(k[t]), gpu.Buffer.of(v[t])
+        check(L.cj_qk_prep(qb.h, kb.h, vb.h, kc.h, vc.h, 0, 0, P.rope_b.h, P.tab.h, 0, heads, kv, hd, 0, f(EPS), 0, t), "qk prep")
+    turned_q = qb.download(np.float32, heads * hd).reshape(heads, hd)
+    # two products and a sum in f32 there, each rounded: 2^-23 of |a| + |b| at most
+    size = np.abs(q[-1]).astype(np.float64)
+    size = size + np.roll(size, hd // 2, -1)
+    assert (np.abs(turned_q - got[-1]) <= 2.0 ** -23 * size).all()
+    check(L.cj_attend(part.h, out.h, qb.h, kc.h, vc.h, P.tab.h, 0, cnt.h, heads, kv, hd, count, 0, 512, f(1 / math.sqrt(hd))), "attend")
+    ours, scale = P.attend([(0, count - 1, 0, 1)], turned_q[None])
+    # the codes' errors lie evenly within half a step, one apart from the other: a score is off by step x |q| x scale / sqrt(12)
+    # in the root mean square, and a channel by the root of the sum of p^2 x ((that x |v|)^2 + step_v^2 / 12), where the sum of
+    # p^2 is the largest p at most; seven times that, and fp16's 2^-11 of a value, over 4096 values
+    there = out.download(np.float32, heads * hd).reshape(heads, hd)
+    ks, vs = (P.ref.steps(0, n).max(0) for n in ("k", "v"))
+    kk, vv = P.ref.values(0, "k", 0, count), P.ref.values(0, "v", 0, count)
+    for h in range(heads):
+        g, x = h * kv // heads, turned_q[h].astype(np.float64)
+        s = scale * kk[:, g] @ x
+        p = np.exp(s - s.max())
+        p /= p.sum()
+        big = np.abs(vv[:, g]).max()
+        sd = math.sqrt(p.max()) * math.hypot(ks[g] * np.linalg.norm(x) * scale / math.sqrt(12) * big, vs[g] / math.sqrt(12))
+        half = 2.0 ** -11 * (1 + scale * np.abs(x).sum() * np.abs(kk[:, g]).max()) * big
+        assert (np.abs(ours[0, h] - there[h]) <= 7 * sd + half).all(), h
+
+
 @pytest.mark.parametrize("rows,count", [(1, 100), (1, 2049), (12, 2049), (200, 300)])
 def test_out_may_be_q(gpu, rows, count):
     rng = np.random.default_rng(rows)
