@@ -1020,33 +1020,15 @@ DEV void kv8_attend_c128(const cj_kv8_args &a) {
     const int w0 = min(c0 + wv * 32, cols - 1), w1 = min(c0 + wv * 32 + 31, cols - 1), c = min(c0 + wv * 32 + n, cols - 1), ri = c / grp;
     const int wfirst = g.pos + w0 / grp, wlast = g.pos + w1 / grp, last = g.pos + ri, first = a.window > 0 ? last + 1 - a.window : 0;
     const int wlow = a.window > 0 ? wfirst + 1 - a.window : 0;   // the first position that any column of the wave sees
-    h16x8 qh[KS], ql[KS];
-    float cs;
+    float qx[KS][8], top = 0, cs;   // (requested before the first page, whose way they then share)
     {
-        float x[KS][8], top = 0;
         const float *src = a.q + (int64_t)(g.row + ri) * a.q_stride + (int64_t)(h * grp + c % grp) * HD + hf * 8;
 #pragma unroll
         for (int k = 0; k < KS; k++) {
-            *(f32x4 *)&x[k][0] = *(const f32x4 *)(src + 16 * k);
-            *(f32x4 *)&x[k][4] = *(const f32x4 *)(src + 16 * k + 4);
-#pragma unroll
-            for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[k][i]));
-        }
-        int u, v;
-        swap32(__float_as_int(top), u, v);
-        const int e = kv8_q_exponent(fmaxf(__int_as_float(u), __int_as_float(v)));
-        const float sign = a.scale < 0 ? -1.0f : 1.0f;
-        cs = ldexpf(a.scale * sign * KV8_LOG2E, e - 14);
-#pragma unroll
-        for (int k = 0; k < KS; k++) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[k][i] = ldexpf(x[k][i] * sign, 14 - e);
-            kv8_halves(x[k], qh[k], ql[k]);
+            *(f32x4 *)&qx[k][0] = *(const f32x4 *)(src + 16 * k);
+            *(f32x4 *)&qx[k][4] = *(const f32x4 *)(src + 16 * k + 4);
         }
     }
-    f32x16 o[DT] = {};
-    float M = -INFINITY, L = 0;
-
     // staging: thread t moves words t, t + 256, .. of the page's K and V codes
     u32x4 kr[CH], vr[CH];
     f32x2 ksn, vsn;
@@ -1081,6 +1063,27 @@ DEV void kv8_attend_c128(const cj_kv8_args &a) {
         }
     };
     load(p0);
+    h16x8 qh[KS], ql[KS];
+    {
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(qx[k][i]));
+        int u, v;
+        swap32(__float_as_int(top), u, v);
+        const int e = kv8_q_exponent(fmaxf(__int_as_float(u), __int_as_float(v)));
+        const float sign = a.scale < 0 ? -1.0f : 1.0f;
+        cs = ldexpf(a.scale * sign * KV8_LOG2E, e - 14);
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) qx[k][i] = ldexpf(qx[k][i] * sign, 14 - e);
+            kv8_halves(qx[k], qh[k], ql[k]);
+        }
+    }
+    f32x16 o[DT] = {};
+    float M = -INFINITY, L = 0;
+
     store(0);
     f32x2 ks = ksn, vs = vsn;
     if (bad) ks[0] = ks[1] = __uint_as_float(0x7fc00000u);

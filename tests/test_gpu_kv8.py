@@ -629,6 +629,38 @@ def test_out_may_be_q(gpu, rows, count):
         assert "part" in gpu.native.last_error()
 
 
+def test_two_threads_with_a_workspace_each(gpu):
+    """Calls of two threads land on the one stream in any order; each thread's results are those of its calls alone."""
+    import threading
+    heads, kv, hd, L = 32, 8, 128, gpu.native.lib()
+    work = []
+    for seed in (1, 2):
+        rng = np.random.default_rng(seed)
+        P = Pages(gpu, heads, kv, hd, 2, 33, seed=seed)
+        P.append([(0, 0, 0, 2049), (1, 0, 2049, 700)], *rows_of(rng, 2749, heads, kv, hd))
+        q = rows_of(rng, 8, heads, kv, hd)[0]
+        segs = [(0, 2045, 0, 4), (1, 696, 4, 4)]
+        need = L.cj_kv8_attend_bytes(2, 4, 2049, heads, kv, hd, 0)
+        assert need > 0
+        work.append((P, P.attend(segs, q, max_count=2049)[0], P.segs(segs), gpu.Buffer.of(q), gpu.Buffer(need),
+                     gpu.Buffer(q.nbytes)))
+    wrong = []
+
+    def run(P, want, sb, qb, part, out):
+        for _ in range(30):
+            rc = L.cj_kv8_attend(out.h, qb.h, P.planes[0].h, P.planes[1].h, P.tab.h, sb.h, part.h, 2, 4, 8, 2049, P.pool, 2, 33,
+                                 heads, kv, hd, heads * hd, heads * hd, 0, ctypes.c_float(1 / math.sqrt(hd)), 0)
+            if rc or not np.array_equal(out.download(np.float32, want.size).reshape(want.shape), want):
+                wrong.append(rc)
+
+    threads = [threading.Thread(target=run, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 def test_refusals(gpu):
     """Arguments that the host refuses before anything is launched."""
     L, ARG = gpu.native.lib(), gpu.native.CJ_ERR_ARG
