@@ -998,7 +998,7 @@ DEV void kv8_attend_c32(const cj_kv8_args &a) {
 // 128, in 985 us are 1.12 PFLOP/s of f16 products (two for each one of the
 // attention's, whose 560 TFLOP/s that makes) at 1.8 GHz, where an 8192^3 f16
 // product of the library reaches 1.15. In a 128-position window (16 prompts of
-// up to 300 rows, 64 / 8 heads of 64: 36 us) the softmax's VALU work.
+// up to 300 rows, 64 / 8 heads of 64: 35 us) the softmax's VALU work.
 #define KV8_MANY 128
 template <int HD>
 DEV void kv8_attend_c128(const cj_kv8_args &a) {
